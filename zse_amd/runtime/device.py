@@ -20,8 +20,9 @@ F32 = "float32"
 BF16 = "bfloat16"
 I32 = "int32"
 F64 = "float64"
-ITEMSIZE = {F32: 4, BF16: 2, I32: 4, F64: 8}
-NUMPY_OF = {F32: np.float32, BF16: np.uint16, I32: np.int32, F64: np.float64}
+U8 = "uint8"
+ITEMSIZE = {F32: 4, BF16: 2, I32: 4, F64: 8, U8: 1}
+NUMPY_OF = {F32: np.float32, BF16: np.uint16, I32: np.int32, F64: np.float64, U8: np.uint8}
 DTYPE_ALIASES = {"float32": F32, "fp32": F32, "f32": F32, "bfloat16": BF16, "bf16": BF16}
 
 
@@ -237,6 +238,9 @@ KERNEL_SIGNATURES = {
                                  _I, _I, _VP, _I, _VP, _I, _I, _I, _I, _VP, _I, _VP],
     "zk_gdelta_gates": [_VP, _I, _I, _I, _VP, _VP, _VP, _VP, _VP, _I, _I, _VP],
     "zk_gdelta": [_VP, _I, _I, _I, _VP, _I, _VP, _VP, _VP, _VP, _I, _I, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _F, _VP],
+    "zk_rope_cache_write_q8": [_VP, _I, _VP, _I, _VP, _I, _VP, _VP, _VP, _I, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, _VP],
+    "zk_cache_read_q8": [_VP, _VP, _VP, _VP, _I, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, _I, _I, _VP],
+    "zk_attention_q8": [_VP, _I, _VP, _VP, _VP, _VP, _I, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, _F, _F, _I, _I, _VP, _SZ, _VP],
 }
 # present only in the bf16 library
 BF16_KERNEL_SIGNATURES = {
@@ -356,6 +360,10 @@ class KernelLibrary:
         self.zk_mlstm_scan_floats = self._dll.zk_mlstm_scan_floats
         self._dll.zk_conv_rows_most_taps.restype, self._dll.zk_conv_rows_most_taps.argtypes = C.c_int, []
         self.zk_conv_rows_most_taps = self._dll.zk_conv_rows_most_taps
+        self._dll.zk_cache_q8_bytes.restype, self._dll.zk_cache_q8_bytes.argtypes = C.c_size_t, [_I] * 4
+        self.zk_cache_q8_bytes = self._dll.zk_cache_q8_bytes
+        self._dll.zk_attention_q8_workspace.restype, self._dll.zk_attention_q8_workspace.argtypes = C.c_size_t, [_I] * 5
+        self.zk_attention_q8_workspace = self._dll.zk_attention_q8_workspace
         if dtype == BF16:
             self._dll.zk_gdelta_token_supports.restype, self._dll.zk_gdelta_token_supports.argtypes = C.c_int, [_I]
             self.zk_gdelta_token_supports = self._dll.zk_gdelta_token_supports
@@ -652,7 +660,7 @@ class Runtime:
         arr = np.ascontiguousarray(arr)
         if dtype is None:
             dtype = {np.dtype(np.float32): F32, np.dtype(np.int32): I32, np.dtype(np.uint16): BF16,
-                     np.dtype(np.float64): F64}[arr.dtype]
+                     np.dtype(np.float64): F64, np.dtype(np.uint8): U8}[arr.dtype]
         t = self.empty(arr.shape, dtype)
         if t.nbytes != arr.nbytes:
             raise ValueError(f"{arr.dtype} array does not store {dtype}")
