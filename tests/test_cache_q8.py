@@ -53,7 +53,9 @@ def test_read_refuses(k, change, says):
     (dict(R=-1), "bad sizes"), (dict(max_ctx=-5), "bad sizes"), (dict(window=-1), "bad sizes"), (dict(nh=0), "bad sizes"),
     (dict(nh=9), "multiple"), (dict(q_stride=1023), "overlap"), (dict(nh=70000, q_stride=70000 * 128), "too many"),
     (dict(max_ctx=129), "longer than the table"), (dict(softcap=-1.0), "softcap"), (dict(q=None), "null"), (dict(out=None), "null"),
-    (dict(ctx_len=None), "null"), (dict(block_table=None), "null")])
+    (dict(ctx_len=None), "null"), (dict(block_table=None), "null"), (dict(R=70000), "too many"), (dict(num_pages=1 << 30), "too many pages"),
+    (dict(max_ctx=20000, max_blocks=2000, workspace=None), "no workspace"), (dict(max_ctx=20000, max_blocks=2000, workspace=A + 4), "multiple of 16"),
+    (dict(max_ctx=20000, max_blocks=2000, workspace_bytes=1000), "too small")])
 def test_attention_refuses(k, change, says):
     from zse_amd.runtime.device import DeviceError
     with pytest.raises(DeviceError, match=f"zk_attention_q8.*{says}"):
@@ -78,6 +80,15 @@ def test_bytes(k):
     assert k.zk_cache_q8_bytes(1 << 20, 16, 256, 128) == (1 << 20) * 16 * 256 * 128
     for bad in ((0, 4, 128, 16), (3, 0, 128, 16), (3, 4, 0, 16), (3, 4, 257, 16), (3, 4, 128, 20)):
         assert k.zk_cache_q8_bytes(*bad) == 0
+
+
+def test_workspace(k):
+    most = k.zk_attention_q8_workspace(64, 8, 128, 8192, 8192)
+    assert most > 0
+    for less in ((63, 8, 128, 8192, 8192), (64, 8, 128, 4000, 8192), (64, 7, 128, 8192, 8192), (64, 8, 64, 8192, 8192)):
+        assert k.zk_attention_q8_workspace(*less) < most
+    for none in ((0, 8, 128, 8192, 8192), (64, 0, 128, 8192, 8192), (64, 8, 257, 8192, 8192), (64, 8, 128, 0, 8192)):
+        assert k.zk_attention_q8_workspace(*none) == 0
 
 
 def test_layout_is_one_to_one():

@@ -14,7 +14,9 @@
 #include "common.h"
 #include "packed_call.h"
 
+#include <algorithm>
 #include <cfloat>
+#include <climits>
 
 extern "C" int zk_steplist_register(const char* name, int nargs, void* fn);
 #define ZK_ENTER(fn) \
@@ -190,60 +192,357 @@ __global__ __launch_bounds__(256) void read_q8_kernel(const uint8_t* __restrict_
 }
 
 // ---------------------------------------------------------------- attended to
-// One wave a (request, head): 64 keys at a time, a lane a key for the scores, lanes over the channels for the values.
+// Scores and outputs by 16 x 16 matrix products whose columns are the query heads of one key head (16 at a time) and whose rows
+// are keys, then channels: S = K Q' over channels, O' = V' P over keys.  A lane of S holds four neighbouring keys of one head,
+// and that is the operand that O' takes: weights stay in registers.  Codes are whole in bfloat16 (8 bits of mantissa), so a
+// key's scale multiplies its score, a value's scale its weight.
+//
+// A block (four waves) takes a chunk of keys at absolute positions, a wave pairs of pieces of 16 in turn; the running maximum, the
+// sum and O' of the four waves are joined in LDS, the chunks' results by a second kernel.  The chunk follows from the width
+// of the table alone, so that a request's sums are cut alike whoever shares its step.
+struct Q8Attention {
+  const act_t* q;
+  const uint8_t *kcodes, *vcodes;
+  const float* scales;
+  const int *block_table, *ctx_len;
+  act_t* out;
+  float *part_o, *part_ml;          // [R][nh][splits][channels, filled up] and [..][2]
+  int q_stride, max_blocks, max_ctx, nh, nkv, hd, pieces, num_pages, window, chunk, q_whole;
+  float k1, k2, c2;                 // z log2(e) = k1 dot, or c2 tanh(k2 dot)
+};
+
+typedef float q8_f4 __attribute__((ext_vector_type(4)));
+typedef unsigned q8_u4 __attribute__((ext_vector_type(4)));
+#if ZSE_ACT_BF16
+typedef __bf16 q8_b8 __attribute__((ext_vector_type(8)));
+typedef __bf16 q8_b2 __attribute__((ext_vector_type(2)));
+#endif
+
+// Four codes as four numbers of the type that the products take.
 template <int FMT>
-__global__ __launch_bounds__(64) void attention_q8_kernel(const act_t* __restrict__ q, int q_stride, const uint8_t* __restrict__ kcodes,
-                                                          const uint8_t* __restrict__ vcodes, const float* __restrict__ scales,
-                                                          const int* __restrict__ block_table, int max_blocks,
-                                                          const int* __restrict__ ctx_len, act_t* __restrict__ out, int max_ctx, int nh,
-                                                          int nkv, int hd, int bs, int num_pages, float scale, float softcap, int window) {
-  __shared__ float s_p[64];
-  __shared__ size_t s_at[64];
-  __shared__ int s_page[64];
-  const int r = blockIdx.x, head = blockIdx.y, lane = threadIdx.x, kvh = head / (nh / nkv), blocks = q8_blocks(hd), pieces = bs / Q8_PIECE;
-  const int ctx = min(ctx_len[r], max_ctx), first = window > 0 ? max(0, ctx - window) : 0;
-  const act_t* row = q + (size_t)r * q_stride + (size_t)head * hd;
-  float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int j0 = first; j0 < ctx; j0 += 64) {
-    const int j = j0 + lane;
-    const int page = j < ctx ? block_table[(size_t)r * max_blocks + j / bs] : -1;
-    float z = -INFINITY, vs = 0.f;
-    size_t at = 0;
-    const bool seen = page >= 0 && page < num_pages;
-    if (seen) {
-      const int off = j % bs;
-      at = q8_piece(page, off / Q8_PIECE, kvh, nkv, pieces, blocks);
-      float dot = 0.f;
-      for (int c = 0; c < hd; c++)
-        dot += to_f32(row[c]) * q8_number<FMT>(kcodes[at + c / 64 * Q8_BYTES + q8_key_at(off % Q8_PIECE, c % 64)]);
-      z = dot * scales[q8_scale(page, kvh, nkv, bs, 0) + off] * scale;
-      if (softcap > 0.f) z = softcap * tanhf(z / softcap);
-      vs = scales[q8_scale(page, kvh, nkv, bs, 1) + off];
-    }
-    const float bad = wave_max_whole(seen && z != z ? 1.f : 0.f);
-    const float now = fmaxf(m, wave_max_whole(z)), base = now == -INFINITY ? 0.f : now;
-    const float keep = expf(m - base);
-    float p = seen ? expf(z - base) : 0.f;
-    if (bad > 0.f) p = __int_as_float(0x7fc00000);
-    l = l * keep + wave_sum_whole(p);
-    m = now;
-    __syncthreads();
-    s_p[lane] = seen ? p * vs : 0.f;
-    s_at[lane] = at;
-    s_page[lane] = seen ? j % bs % Q8_PIECE : -1;
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      if (lane + 64 * e >= hd) continue;
-      float sum = 0.f;
-      for (int i = 0; i < 64; i++)
-        if (s_page[i] >= 0) sum += s_p[i] * q8_number<FMT>(vcodes[s_at[i] + e * Q8_BYTES + q8_value_at(s_page[i], lane)]);
-      acc[e] = acc[e] * keep + sum;
+__device__ __forceinline__ void q8_floats(unsigned codes, float (&x)[4]) {
+#ifdef __HIP_DEVICE_COMPILE__
+  if constexpr (FMT == 0) {
+    x[0] = (float)(int)(int8_t)codes;
+    x[1] = (float)(int)(int8_t)(codes >> 8);
+    x[2] = (float)(int)(int8_t)(codes >> 16);
+    x[3] = (float)((int)codes >> 24);
+  } else {
+    x[0] = __builtin_amdgcn_cvt_f32_fp8((int)codes, 0);
+    x[1] = __builtin_amdgcn_cvt_f32_fp8((int)codes, 1);
+    x[2] = __builtin_amdgcn_cvt_f32_fp8((int)codes, 2);
+    x[3] = __builtin_amdgcn_cvt_f32_fp8((int)codes, 3);
+  }
+#endif
+}
+#if ZSE_ACT_BF16
+template <int FMT>
+__device__ __forceinline__ void q8_halves(unsigned codes, unsigned& lo, unsigned& hi) {
+#ifdef __HIP_DEVICE_COMPILE__
+  if constexpr (FMT == 0) {
+    float x[4];                       // whole numbers up to 127: the upper halves hold them
+    q8_floats<FMT>(codes, x);
+    lo = __builtin_amdgcn_perm(__float_as_uint(x[1]), __float_as_uint(x[0]), 0x07060302);
+    hi = __builtin_amdgcn_perm(__float_as_uint(x[3]), __float_as_uint(x[2]), 0x07060302);
+  } else {
+    lo = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.f, false));
+    hi = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.f, true));
+  }
+#endif
+}
+template <int FMT>
+__device__ __forceinline__ q8_b8 q8_operand(unsigned a, unsigned b) {
+  q8_u4 w;
+  unsigned lo = 0, hi = 0;
+  q8_halves<FMT>(a, lo, hi);
+  w[0] = lo;
+  w[1] = hi;
+  q8_halves<FMT>(b, lo, hi);
+  w[2] = lo;
+  w[3] = hi;
+  return __builtin_bit_cast(q8_b8, w);
+}
+#endif
+
+template <int FMT, int NB, bool CAP, bool DIRECT>
+__global__ __launch_bounds__(256, 2) void attention_q8_kernel(Q8Attention p) {
+#ifdef __HIP_DEVICE_COMPILE__
+  extern __shared__ float s_join[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+  const int group = p.nh / p.nkv, kvh = blockIdx.y % p.nkv, head0 = blockIdx.y / p.nkv * 16, r = blockIdx.z;
+  const int heads = min(16, group - head0), splits = gridDim.x;
+  const int ctx = min(p.ctx_len[r], p.max_ctx), first = p.window > 0 ? max(0, ctx - p.window) : 0;
+  const int from = first / p.chunk * p.chunk + blockIdx.x * p.chunk;
+  const int begin = max(first, from), end = min(ctx, from + p.chunk);
+  const int head = kvh * group + head0 + col;             // this lane's column, if col < heads
+  if (begin >= end) {
+    if (DIRECT)
+      for (int i = threadIdx.x; i < heads * p.hd; i += 256)
+        p.out[((size_t)r * p.nh + kvh * group + head0) * p.hd + i] = from_f32<act_t>(0.f);
+    return;
+  }
+  // lane i: where the chunk's piece i lies; -1 where the table names no page
+  const int p0 = begin / Q8_PIECE, n_pieces = (end + Q8_PIECE - 1) / Q8_PIECE - p0;
+  int piece_at = -1, scale_at = 0;
+  if (lane < n_pieces) {
+    const int i = p0 + lane, page = p.block_table[(size_t)r * p.max_blocks + i / p.pieces];
+    if (page >= 0 && page < p.num_pages) {
+      const int at = page * p.nkv + kvh;
+      piece_at = at * p.pieces + i % p.pieces;
+      scale_at = at * 2 * p.pieces + i % p.pieces;
     }
   }
+  const int n_pairs = (n_pieces + 1) / 2;
+  const int k_lane = col * 64 + g * 16, v_lane = lane * 16;
+  // keys of piece 2 pair + u, and values of both; what is not there is asked for at the cache's beginning and left out below
+  q8_u4 kc[2][NB], vc[2][NB];
+  q8_f4 ks[2], vs[2];
+  auto at_piece = [&](int i, int at) { return i < n_pieces ? max(__builtin_amdgcn_readlane(at, i), 0) : 0; };
+  auto ask_keys = [&](int pair, int u) {
+    const uint8_t* at = p.kcodes + (size_t)at_piece(2 * pair + u, piece_at) * (NB * Q8_BYTES);
+    ks[u] = *(const q8_f4*)(p.scales + (size_t)at_piece(2 * pair + u, scale_at) * Q8_PIECE + 4 * g);
 #pragma unroll
-  for (int e = 0; e < 4; e++)
-    if (lane + 64 * e < hd) out[((size_t)r * nh + head) * hd + lane + 64 * e] = from_f32<act_t>(l == 0.f ? 0.f : acc[e] / l);
+    for (int j = 0; j < NB; j++) kc[u][j] = *(const q8_u4*)(at + j * Q8_BYTES + k_lane);
+  };
+  auto ask_values = [&](int pair) {
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const uint8_t* at = p.vcodes + (size_t)at_piece(2 * pair + u, piece_at) * (NB * Q8_BYTES);
+      vs[u] = *(const q8_f4*)(p.scales + ((size_t)at_piece(2 * pair + u, scale_at) + p.pieces) * Q8_PIECE + 4 * g);
+#pragma unroll
+      for (int j = 0; j < NB; j++) vc[u][j] = *(const q8_u4*)(at + j * Q8_BYTES + v_lane);
+    }
+  };
+  if (wave < n_pairs) {
+    ask_keys(wave, 0);
+    ask_keys(wave, 1);
+    ask_values(wave);
+  }
+
+  // the queries: channels 64 j + 16 g .. + 15 of head col
+#if ZSE_ACT_BF16
+  q8_b8 qf[NB][2];
+#else
+  float qf[NB][16];
+#endif
+  {
+    const act_t* row = p.q + (size_t)r * p.q_stride + (size_t)head * p.hd;
+#pragma unroll
+    for (int j = 0; j < NB; j++)
+#pragma unroll
+      for (int s = 0; s < 2; s++) {
+        const int c0 = 64 * j + 16 * g + 8 * s;
+        typedef act_t a8 __attribute__((ext_vector_type(8)));
+        a8 x;
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = from_f32<act_t>(0.f);
+        if (col < heads) {
+          if (p.q_whole) {
+            if (c0 < p.hd) x = *(const a8*)(row + c0);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+              if (c0 + e < p.hd) x[e] = row[c0 + e];
+          }
+        }
+#if ZSE_ACT_BF16
+        qf[j][s] = x;
+#else
+#pragma unroll
+        for (int e = 0; e < 8; e++) qf[j][8 * s + e] = x[e];
+#endif
+      }
+  }
+
+  float m = -INFINITY, l = 0.f;
+  q8_f4 o[NB * 4];
+#pragma unroll
+  for (int t = 0; t < NB * 4; t++) o[t] = q8_f4{0.f, 0.f, 0.f, 0.f};
+  for (int pair = wave; pair < n_pairs; pair += 4) {
+    // scores of head col: keys 16 (p0 + 2 pair + u) + 4 g + i
+    float z[2][4];
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      q8_f4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < NB; j++) {
+#if ZSE_ACT_BF16
+        s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q8_operand<FMT>(kc[u][j][0], kc[u][j][1]), qf[j][0], s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q8_operand<FMT>(kc[u][j][2], kc[u][j][3]), qf[j][1], s, 0, 0, 0);
+#else
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+          float x[4];
+          q8_floats<FMT>(kc[u][j][w], x);
+#pragma unroll
+          for (int e = 0; e < 4; e++) s = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], qf[j][4 * w + e], s, 0, 0, 0);
+        }
+#endif
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float dot = s[i] * ks[u][i];
+        if constexpr (CAP) {
+#if ZSE_ACT_BF16
+          z[u][i] = p.c2 - 2.f * p.c2 * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(p.k2 * dot) + 1.f);
+#else
+          z[u][i] = p.c2 * tanhf(p.k2 * dot);
+#endif
+        } else z[u][i] = p.k1 * dot;
+      }
+    }
+    if (pair + 4 < n_pairs) {
+      ask_keys(pair + 4, 0);
+      ask_keys(pair + 4, 1);
+    }
+    // keys outside of [begin, end) and in pages that are not there
+    const int key0 = (p0 + 2 * pair) * Q8_PIECE;
+    const int at0 = __builtin_amdgcn_readlane(piece_at, 2 * pair);
+    const int at1 = 2 * pair + 1 < n_pieces ? __builtin_amdgcn_readlane(piece_at, 2 * pair + 1) : -1;
+    const bool whole = key0 >= begin && key0 + 2 * Q8_PIECE <= end && at0 >= 0 && at1 >= 0;
+    if (!whole) {
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        unsigned mask = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int key = key0 + u * Q8_PIECE + 4 * g + i;
+          const bool seen = key >= begin && key < end && (u ? at1 : at0) >= 0;
+          mask |= seen ? 255u << (8 * i) : 0u;
+          z[u][i] = seen ? z[u][i] : -INFINITY;
+          vs[u][i] = seen ? vs[u][i] : 0.f;
+        }
+        // a code that is no number would meet a weight of zero
+#pragma unroll
+        for (int j = 0; j < NB; j++)
+#pragma unroll
+          for (int b = 0; b < 4; b++) vc[u][j][b] &= mask;
+      }
+    }
+    float top = z[0][0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) top = fmaxf(top, z[i / 4][i % 4]);
+    const float m_new = fmaxf(m, wave_max16_32(top)), base = m_new == -INFINITY ? 0.f : m_new;
+    if (__any(m_new != m)) {
+      const float keep = __builtin_amdgcn_exp2f(m - base);
+      l *= keep;
+#pragma unroll
+      for (int t = 0; t < NB * 4; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[t][i] *= keep;
+      m = m_new;
+    }
+    float w[2][4];
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float e = __builtin_amdgcn_exp2f(z[u][i] - base);
+        l += e;
+        w[u][i] = e * vs[u][i];
+      }
+#if ZSE_ACT_BF16
+    // the weights round to the values' type (half a step of 2^-8 each); their sum does not
+    q8_b8 pb;
+#pragma unroll
+    for (int e = 0; e < 8; e++) pb[e] = (__bf16)w[e / 4][e % 4];
+#pragma unroll
+    for (int j = 0; j < NB; j++)
+#pragma unroll
+      for (int b = 0; b < 4; b++)
+        o[4 * j + b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q8_operand<FMT>(vc[0][j][b], vc[1][j][b]), pb, o[4 * j + b], 0, 0, 0);
+#else
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+      for (int j = 0; j < NB; j++)
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+          float x[4];
+          q8_floats<FMT>(vc[u][j][b], x);
+#pragma unroll
+          for (int i = 0; i < 4; i++) o[4 * j + b] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], w[u][i], o[4 * j + b], 0, 0, 0);
+        }
+#endif
+    if (pair + 4 < n_pairs) ask_values(pair + 4);
+  }
+  l = wave_add16_32(l);
+
+  // the four waves' results: [wave][head][channels, then maximum and sum]
+  constexpr int ROW = NB * 64 + 4;
+  if (col < heads) {
+    float* mine = s_join + (wave * heads + col) * ROW;
+#pragma unroll
+    for (int t = 0; t < NB * 4; t++) *(q8_f4*)(mine + 16 * t + 4 * g) = o[t];
+    if (g == 0) {
+      mine[NB * 64] = m;
+      mine[NB * 64 + 1] = l;
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < heads * NB * 64; i += 256) {
+    const int h = i / (NB * 64), c = i % (NB * 64);
+    float mw[4], most = -INFINITY, sum = 0.f, x = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) most = fmaxf(most, mw[w] = s_join[(w * heads + h) * ROW + NB * 64]);
+    const float base = most == -INFINITY ? 0.f : most;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      const float f = __builtin_amdgcn_exp2f(mw[w] - base);
+      sum += f * s_join[(w * heads + h) * ROW + NB * 64 + 1];
+      x += f * s_join[(w * heads + h) * ROW + c];
+    }
+    const size_t hd_at = (size_t)r * p.nh + kvh * group + head0 + h;
+    if (DIRECT) {
+      if (c < p.hd) p.out[hd_at * p.hd + c] = from_f32<act_t>(sum == 0.f ? 0.f : x / sum);
+    } else {
+      const size_t part = hd_at * splits + blockIdx.x;
+      p.part_o[part * (NB * 64) + c] = x;
+      if (c == 0) {
+        p.part_ml[part * 2] = most;
+        p.part_ml[part * 2 + 1] = sum;
+      }
+    }
+  }
+#endif
+}
+
+// Joins the chunks' results of a (head, request): four channels a thread, the chunks dealt to as many groups of threads as there are.
+template <int NB>
+__global__ __launch_bounds__(256) void attention_q8_join_kernel(Q8Attention p, int splits) {
+  constexpr int LANES = NB * 16, GROUPS = 256 / LANES;
+  __shared__ float s_o[GROUPS][NB * 64], s_l[GROUPS];
+  const int head = blockIdx.x, r = blockIdx.y, group = threadIdx.x / LANES, at = threadIdx.x % LANES;
+  const int ctx = min(p.ctx_len[r], p.max_ctx), first = p.window > 0 ? max(0, ctx - p.window) : 0;
+  const int n = ctx > 0 ? (ctx + p.chunk - 1) / p.chunk - first / p.chunk : 0;
+  const size_t row = ((size_t)r * p.nh + head) * splits;
+  float most = -INFINITY;
+  for (int i = threadIdx.x & 63; i < n; i += 64) most = fmaxf(most, p.part_ml[(row + i) * 2]);
+  most = wave_max_whole(most);
+  const float base = most == -INFINITY ? 0.f : most;
+  float l = 0.f;
+  q8_f4 o = {0.f, 0.f, 0.f, 0.f};
+  if (group < GROUPS) {
+    for (int i = group; i < n; i += GROUPS) {
+      const float f = exp2f(p.part_ml[(row + i) * 2] - base);
+      const q8_f4 x = *(const q8_f4*)(p.part_o + (row + i) * (NB * 64) + at * 4);
+      l += f * p.part_ml[(row + i) * 2 + 1];
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[e] += f * x[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) s_o[group][at * 4 + e] = o[e];
+    if (at == 0) s_l[group] = l;
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < p.hd; c += 256) {
+    float x = 0.f, sum = 0.f;
+    for (int w = 0; w < GROUPS; w++) {
+      x += s_o[w][c];
+      sum += s_l[w];
+    }
+    p.out[((size_t)r * p.nh + head) * p.hd + c] = from_f32<act_t>(sum == 0.f ? 0.f : x / sum);
+  }
 }
 
 // ---------------------------------------------------------------- entry points
@@ -267,6 +566,17 @@ static int q8_refuses(const char* who, const void* kcodes, const void* vcodes, c
     constexpr int FMT = 1;         \
     call;                          \
   }
+
+// Keys of a partial result, by what a request's table can hold: see attention_q8_kernel.
+#ifndef Q8_CHUNK
+#define Q8_CHUNK 256
+#endif
+static int q8_chunk(int table_tokens) { return Q8_CHUNK; }
+// Chunks that a request of up to max_ctx tokens may meet.
+static int q8_splits(int max_ctx, int window, int chunk) {
+  const int all = (max_ctx + chunk - 1) / chunk;
+  return window > 0 ? (int)std::min<long long>(all, ((long long)window + chunk - 2) / chunk + 1) : all;
+}
 
 extern "C" {
 
@@ -322,8 +632,12 @@ int zk_cache_read_q8(const void* kcodes, const void* vcodes, const float* scales
   return zk_launch_status("zk_cache_read_q8");
 }
 
-// Bytes of workspace of zk_attention_q8 for R requests of up to max_ctx tokens whose table reaches table_tokens.
-size_t zk_attention_q8_workspace(int R, int nh, int hd, int max_ctx, int table_tokens) { return 0; }
+// Bytes of workspace of zk_attention_q8 for R requests of up to max_ctx tokens whose table reaches table_tokens (more of either is
+// more: a caller may ask for its largest).
+size_t zk_attention_q8_workspace(int R, int nh, int hd, int max_ctx, int table_tokens) {
+  if (R <= 0 || nh <= 0 || hd <= 0 || hd > 256 || max_ctx <= 0) return 0;
+  return (size_t)R * nh * q8_splits(max_ctx, 0, q8_chunk(table_tokens)) * (q8_blocks(hd) * Q8_BLOCK + 2) * sizeof(float);
+}
 
 // Attention of one token a request, the last of its ctx_len[r], over its cache: z_j = scale q.k_j (softcap > 0: softcap
 // tanh(z_j / softcap)) for j from max(0, ctx - window) on (all without a window), out = sum softmax(z)_j v_j.  q: row r at r * q_stride;
@@ -335,14 +649,77 @@ int zk_attention_q8(const void* q, int q_stride, const void* kcodes, const void*
   Q8_REQUIRE_CACHE("zk_attention_q8");
   ZK_REQUIRE(R >= 0 && max_ctx >= 0 && window >= 0 && max_blocks >= 0 && nh > 0, "zk_attention_q8: bad sizes");
   ZK_REQUIRE(nh % nkv == 0, "zk_attention_q8: query heads must be a multiple of key heads");
-  ZK_REQUIRE(nh <= 65535 && q_stride >= nh * hd, "zk_attention_q8: rows overlap, or too many heads");
+  ZK_REQUIRE(nh <= 65535 && R <= 65535, "zk_attention_q8: too many heads or requests");
+  ZK_REQUIRE(q_stride >= (long long)nh * hd, "zk_attention_q8: rows overlap");
   ZK_REQUIRE(max_ctx <= (long long)max_blocks * bs, "zk_attention_q8: contexts longer than the table");
+  ZK_REQUIRE((long long)num_pages * nkv * 2 * (bs / Q8_PIECE) < (1ll << 31), "zk_attention_q8: too many pages");
   ZK_REQUIRE(softcap >= 0.f, "zk_attention_q8: softcap must not be negative");
   if (R == 0) return 0;
   ZK_REQUIRE(q && out && ctx_len && (block_table || max_ctx == 0), "zk_attention_q8: null argument");
-  Q8_FORMAT((attention_q8_kernel<FMT><<<dim3(R, nh), 64, 0, (hipStream_t)stream>>>(
-      (const act_t*)q, q_stride, (const uint8_t*)kcodes, (const uint8_t*)vcodes, scales, block_table, max_blocks, ctx_len, (act_t*)out,
-      max_ctx, nh, nkv, hd, bs, num_pages, scale, softcap, window)))
+  Q8Attention p;
+  p.chunk = q8_chunk((int)std::min<long long>((long long)max_blocks * bs, INT_MAX));
+  const int splits = q8_splits(max_ctx, window, p.chunk), blocks = q8_blocks(hd);
+  const size_t row = (size_t)R * nh * splits;
+  if (splits > 1) {
+    ZK_REQUIRE(workspace && (uintptr_t)workspace % 16 == 0, "zk_attention_q8: no workspace, or not at a multiple of 16");
+    ZK_REQUIRE(workspace_bytes >= row * (blocks * Q8_BLOCK + 2) * sizeof(float), "zk_attention_q8: the workspace is too small");
+  }
+  p.q = (const act_t*)q;
+  p.kcodes = (const uint8_t*)kcodes;
+  p.vcodes = (const uint8_t*)vcodes;
+  p.scales = scales;
+  p.block_table = block_table;
+  p.ctx_len = ctx_len;
+  p.out = (act_t*)out;
+  p.part_o = (float*)workspace;
+  p.part_ml = splits > 1 ? (float*)workspace + row * blocks * Q8_BLOCK : nullptr;
+  p.q_stride = q_stride;
+  p.max_blocks = max_blocks;
+  p.max_ctx = max_ctx;
+  p.nh = nh;
+  p.nkv = nkv;
+  p.hd = hd;
+  p.pieces = bs / Q8_PIECE;
+  p.num_pages = num_pages;
+  p.window = window;
+  // queries by loads of eight, where heads and rows are whole such pieces
+  p.q_whole = hd % 8 == 0 && q_stride % 8 == 0 && (uintptr_t)q % (8 * sizeof(act_t)) == 0;
+  const float log2e = 1.44269504088896f;
+  p.k1 = scale * log2e;
+#if ZSE_ACT_BF16
+  p.k2 = softcap > 0.f ? 2.f * scale / softcap * log2e : 0.f;
+#else
+  p.k2 = softcap > 0.f ? scale / softcap : 0.f;
+#endif
+  p.c2 = softcap * log2e;
+  const int group = nh / nkv, tiles = (group + 15) / 16;
+  const dim3 grid(splits, nkv * tiles, R);
+  const size_t lds = (size_t)4 * std::min(group, 16) * (blocks * Q8_BLOCK + 4) * sizeof(float);
+#define Q8_ATTEND(FMT, NB)                                                                                             \
+  do {                                                                                                                 \
+    const auto kernel = softcap > 0.f ? (splits > 1 ? attention_q8_kernel<FMT, NB, true, false> : attention_q8_kernel<FMT, NB, true, true>)    \
+                                      : (splits > 1 ? attention_q8_kernel<FMT, NB, false, false> : attention_q8_kernel<FMT, NB, false, true>); \
+    if (lds > (64 << 10)) {                                                                                            \
+      const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds); \
+      if (e != hipSuccess) return zk_fail("zk_attention_q8: no room in LDS");                                          \
+    }                                                                                                                  \
+    kernel<<<grid, 256, lds, (hipStream_t)stream>>>(p);                                                                \
+    if (splits > 1) attention_q8_join_kernel<NB><<<dim3(nh, R), 256, 0, (hipStream_t)stream>>>(p, splits);             \
+  } while (0)
+#define Q8_BY_BLOCKS(FMT)                    \
+  switch (blocks) {                          \
+    case 1: Q8_ATTEND(FMT, 1); break;        \
+    case 2: Q8_ATTEND(FMT, 2); break;        \
+    case 3: Q8_ATTEND(FMT, 3); break;        \
+    default: Q8_ATTEND(FMT, 4); break;       \
+  }
+  if (format == 0) {
+    Q8_BY_BLOCKS(0)
+  } else {
+    Q8_BY_BLOCKS(1)
+  }
+#undef Q8_BY_BLOCKS
+#undef Q8_ATTEND
   return zk_launch_status("zk_attention_q8");
 }
 
