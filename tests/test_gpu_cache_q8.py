@@ -296,7 +296,7 @@ def test_attended(rt, nh, nkv, hd, bs, form, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
-@pytest.mark.parametrize("what", ["holes", "bad_pages", "none", "stride", "max_ctx", "big_scores", "all_equal", "nan_key"])
+@pytest.mark.parametrize("what", ["holes", "bad_pages", "none", "stride", "max_ctx", "no_ctx", "big_scores", "all_equal", "nan_key"])
 def test_attended_otherwise(rt, what, dtype):
     rng = np.random.default_rng(len(what))
     nh, nkv, hd, bs, form = 8, 2, 64, 32, 1
@@ -317,6 +317,8 @@ def test_attended_otherwise(rt, what, dtype):
         stride = nh * hd + 5
     if what == "max_ctx":
         max_ctx = 40
+    if what == "no_ctx":
+        max_ctx, table = 0, table[:, :0]
     if what == "big_scores":
         scale = 50.0
     if what == "all_equal":
@@ -328,8 +330,8 @@ def test_attended_otherwise(rt, what, dtype):
         assert np.isnan(got[3, nh // 2:]).all() and np.isfinite(got[3, :nh // 2]).all()
         c.scales[table[3, 2], 1, 0, 7] = 1.0
         lens, got = lens[:3], got[:3]
-    if what == "max_ctx":
-        lens = [min(n, 40) for n in lens]
+    if what in ("max_ctx", "no_ctx"):
+        lens = [min(n, max_ctx) for n in lens]
     check_attended(c, got, q, table, lens, nh, scale, 0.0, 0, dtype)
 
 

@@ -16,7 +16,6 @@
 
 #include <algorithm>
 #include <cfloat>
-#include <climits>
 
 extern "C" int zk_steplist_register(const char* name, int nargs, void* fn);
 #define ZK_ENTER(fn) \
@@ -264,15 +263,21 @@ __device__ __forceinline__ q8_b8 q8_operand(unsigned a, unsigned b) {
 }
 #endif
 
-template <int FMT, int NB, bool CAP, bool DIRECT>
+template <int FMT, int NB, bool CAP, bool DIRECT, bool ONCE>
 __global__ __launch_bounds__(256, 2) void attention_q8_kernel(Q8Attention p) {
 #ifdef __HIP_DEVICE_COMPILE__
   extern __shared__ float s_join[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
   const int group = p.nh / p.nkv, kvh = blockIdx.y % p.nkv, head0 = blockIdx.y / p.nkv * 16, r = blockIdx.z;
   const int heads = min(16, group - head0), splits = gridDim.x;
+  // neighbouring blocks go to different XCDs: turned by request and head, so that no XCD has one chunk of every request (with eight
+  // chunks 64 requests of uneven lengths took 74 us instead of 59)
+  const int split = (blockIdx.x + blockIdx.y + r) % splits;
+  // without a window the chunk's place in the table does not wait for the request's length
+  int early = -1;
+  if (p.window == 0 && p.max_ctx > 0) early = p.block_table[(size_t)r * p.max_blocks + min((split * (p.chunk / Q8_PIECE) + lane) / p.pieces, p.max_blocks - 1)];
   const int ctx = min(p.ctx_len[r], p.max_ctx), first = p.window > 0 ? max(0, ctx - p.window) : 0;
-  const int from = first / p.chunk * p.chunk + blockIdx.x * p.chunk;
+  const int from = first / p.chunk * p.chunk + split * p.chunk;
   const int begin = max(first, from), end = min(ctx, from + p.chunk);
   const int head = kvh * group + head0 + col;             // this lane's column, if col < heads
   if (begin >= end) {
@@ -285,7 +290,7 @@ __global__ __launch_bounds__(256, 2) void attention_q8_kernel(Q8Attention p) {
   const int p0 = begin / Q8_PIECE, n_pieces = (end + Q8_PIECE - 1) / Q8_PIECE - p0;
   int piece_at = -1, scale_at = 0;
   if (lane < n_pieces) {
-    const int i = p0 + lane, page = p.block_table[(size_t)r * p.max_blocks + i / p.pieces];
+    const int i = p0 + lane, page = p.window == 0 ? early : p.block_table[(size_t)r * p.max_blocks + i / p.pieces];
     if (page >= 0 && page < p.num_pages) {
       const int at = page * p.nkv + kvh;
       piece_at = at * p.pieces + i % p.pieces;
@@ -302,7 +307,7 @@ __global__ __launch_bounds__(256, 2) void attention_q8_kernel(Q8Attention p) {
     const uint8_t* at = p.kcodes + (size_t)at_piece(2 * pair + u, piece_at) * (NB * Q8_BYTES);
     ks[u] = *(const q8_f4*)(p.scales + (size_t)at_piece(2 * pair + u, scale_at) * Q8_PIECE + 4 * g);
 #pragma unroll
-    for (int j = 0; j < NB; j++) kc[u][j] = *(const q8_u4*)(at + j * Q8_BYTES + k_lane);
+    for (int j = 0; j < NB; j++) kc[u][j] = load_maybe_once<ONCE>((const q8_u4*)(at + j * Q8_BYTES + k_lane));
   };
   auto ask_values = [&](int pair) {
 #pragma unroll
@@ -310,7 +315,7 @@ __global__ __launch_bounds__(256, 2) void attention_q8_kernel(Q8Attention p) {
       const uint8_t* at = p.vcodes + (size_t)at_piece(2 * pair + u, piece_at) * (NB * Q8_BYTES);
       vs[u] = *(const q8_f4*)(p.scales + ((size_t)at_piece(2 * pair + u, scale_at) + p.pieces) * Q8_PIECE + 4 * g);
 #pragma unroll
-      for (int j = 0; j < NB; j++) vc[u][j] = *(const q8_u4*)(at + j * Q8_BYTES + v_lane);
+      for (int j = 0; j < NB; j++) vc[u][j] = load_maybe_once<ONCE>((const q8_u4*)(at + j * Q8_BYTES + v_lane));
     }
   };
   if (wave < n_pairs) {
@@ -496,7 +501,7 @@ __global__ __launch_bounds__(256, 2) void attention_q8_kernel(Q8Attention p) {
     if (DIRECT) {
       if (c < p.hd) p.out[hd_at * p.hd + c] = from_f32<act_t>(sum == 0.f ? 0.f : x / sum);
     } else {
-      const size_t part = hd_at * splits + blockIdx.x;
+      const size_t part = hd_at * splits + split;
       p.part_o[part * (NB * 64) + c] = x;
       if (c == 0) {
         p.part_ml[part * 2] = most;
@@ -508,40 +513,58 @@ __global__ __launch_bounds__(256, 2) void attention_q8_kernel(Q8Attention p) {
 }
 
 // Joins the chunks' results of a (head, request): four channels a thread, the chunks dealt to as many groups of threads as there are.
+// What the first round reads is asked for before the request's length is known (one wait for memory instead of three; what lies
+// behind its chunks is never used).
 template <int NB>
 __global__ __launch_bounds__(256) void attention_q8_join_kernel(Q8Attention p, int splits) {
-  constexpr int LANES = NB * 16, GROUPS = 256 / LANES;
-  __shared__ float s_o[GROUPS][NB * 64], s_l[GROUPS];
-  const int head = blockIdx.x, r = blockIdx.y, group = threadIdx.x / LANES, at = threadIdx.x % LANES;
-  const int ctx = min(p.ctx_len[r], p.max_ctx), first = p.window > 0 ? max(0, ctx - p.window) : 0;
-  const int n = ctx > 0 ? (ctx + p.chunk - 1) / p.chunk - first / p.chunk : 0;
+  constexpr int LANES = NB * 16, GROUPS = 256 / LANES, AHEAD = 4;
+  __shared__ float s_o[GROUPS][NB * 64];
+  const int head = blockIdx.x, r = blockIdx.y, lane = threadIdx.x & 63, group = min((int)threadIdx.x / LANES, GROUPS - 1), at = threadIdx.x % LANES;
   const size_t row = ((size_t)r * p.nh + head) * splits;
-  float most = -INFINITY;
-  for (int i = threadIdx.x & 63; i < n; i += 64) most = fmaxf(most, p.part_ml[(row + i) * 2]);
+  const int ctx = min(p.ctx_len[r], p.max_ctx), first = p.window > 0 ? max(0, ctx - p.window) : 0;
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  const f2* ml = (const f2*)p.part_ml + row;
+  const f2 mine = ml[min(lane, splits - 1)];
+  const float* part = p.part_o + row * (NB * 64) + at * 4;
+  q8_f4 x[AHEAD];
+#pragma unroll
+  for (int e = 0; e < AHEAD; e++) x[e] = *(const q8_f4*)(part + (size_t)min(group + e * GROUPS, splits - 1) * (NB * 64));
+  const int n = ctx > 0 ? (ctx + p.chunk - 1) / p.chunk - first / p.chunk : 0;
+  float most = lane < n ? mine[0] : -INFINITY;
+  for (int i = lane + 64; i < n; i += 64) most = fmaxf(most, ml[i][0]);
   most = wave_max_whole(most);
   const float base = most == -INFINITY ? 0.f : most;
-  float l = 0.f;
+  // lane i's factor of chunk i, and the sum of what the wave's lanes hold
+  float f = lane < n ? exp2f(mine[0] - base) : 0.f;
+  float l = lane < n ? f * mine[1] : 0.f;
   q8_f4 o = {0.f, 0.f, 0.f, 0.f};
-  if (group < GROUPS) {
-    for (int i = group; i < n; i += GROUPS) {
-      const float f = exp2f(p.part_ml[(row + i) * 2] - base);
-      const q8_f4 x = *(const q8_f4*)(p.part_o + (row + i) * (NB * 64) + at * 4);
-      l += f * p.part_ml[(row + i) * 2 + 1];
 #pragma unroll
-      for (int e = 0; e < 4; e++) o[e] += f * x[e];
+  for (int e = 0; e < AHEAD; e++) {
+    const int i = group + e * GROUPS;
+    const float w = __shfl(f, i & 63);
+    if (i < n) o += w * x[e];
+  }
+  for (int i0 = AHEAD * GROUPS; i0 < n; i0 += AHEAD * GROUPS) {
+    float w[AHEAD];
+#pragma unroll
+    for (int e = 0; e < AHEAD; e++) {
+      const int i = min(i0 + group + e * GROUPS, n - 1);
+      w[e] = ml[i][0];
+      x[e] = *(const q8_f4*)(part + (size_t)i * (NB * 64));
     }
 #pragma unroll
-    for (int e = 0; e < 4; e++) s_o[group][at * 4 + e] = o[e];
-    if (at == 0) s_l[group] = l;
+    for (int e = 0; e < AHEAD; e++)
+      if (i0 + group + e * GROUPS < n) o += exp2f(w[e] - base) * x[e];
   }
+  for (int i = lane + 64; i < n; i += 64) l += exp2f(ml[i][0] - base) * ml[i][1];
+  l = wave_sum_whole(l);
+  if (threadIdx.x < LANES * GROUPS) *(q8_f4*)&s_o[group][at * 4] = o;
   __syncthreads();
   for (int c = threadIdx.x; c < p.hd; c += 256) {
-    float x = 0.f, sum = 0.f;
-    for (int w = 0; w < GROUPS; w++) {
-      x += s_o[w][c];
-      sum += s_l[w];
-    }
-    p.out[((size_t)r * p.nh + head) * p.hd + c] = from_f32<act_t>(sum == 0.f ? 0.f : x / sum);
+    float y = 0.f;
+#pragma unroll
+    for (int w = 0; w < GROUPS; w++) y += s_o[w][c];
+    p.out[((size_t)r * p.nh + head) * p.hd + c] = from_f32<act_t>(l == 0.f ? 0.f : y / l);
   }
 }
 
@@ -567,14 +590,20 @@ static int q8_refuses(const char* who, const void* kcodes, const void* vcodes, c
     call;                          \
   }
 
-// Keys of a partial result, by what a request's table can hold: see attention_q8_kernel.
-#ifndef Q8_CHUNK
-#define Q8_CHUNK 256
+// Keys of a partial result, by what a request's table can hold.  us by 256, 512 and 1,024 keys (16-bit rows, 8 heads over 4 of 256
+// channels): one request of 4,000 keys 10.8, 12.8, 18.9; 64 of them 98.6, 93.7, 91.4; one of 16,000 15.6, 15.3, 20.8; eight of
+// them 56.3, 49.8, 47.9; one of 60,000 45.1, 33.5, 28.3.  32-bit products take eight times as long for as many keys: by 128, 256
+// and 512, 8 heads over 2 of 128, three requests of up to 700 keys 10.2, 12.9, 19.7; 8 over 4 of 256, one of 16,000 29.4, 25.1, 33.9.
+static int q8_chunk(long long table_tokens) {
+#if ZSE_ACT_BF16
+  return table_tokens < 8192 ? 256 : table_tokens < 32768 ? 512 : 1024;
+#else
+  return table_tokens < 8192 ? 128 : 256;
 #endif
-static int q8_chunk(int table_tokens) { return Q8_CHUNK; }
+}
 // Chunks that a request of up to max_ctx tokens may meet.
 static int q8_splits(int max_ctx, int window, int chunk) {
-  const int all = (max_ctx + chunk - 1) / chunk;
+  const int all = std::max(1, (max_ctx + chunk - 1) / chunk);
   return window > 0 ? (int)std::min<long long>(all, ((long long)window + chunk - 2) / chunk + 1) : all;
 }
 
@@ -657,7 +686,7 @@ int zk_attention_q8(const void* q, int q_stride, const void* kcodes, const void*
   if (R == 0) return 0;
   ZK_REQUIRE(q && out && ctx_len && (block_table || max_ctx == 0), "zk_attention_q8: null argument");
   Q8Attention p;
-  p.chunk = q8_chunk((int)std::min<long long>((long long)max_blocks * bs, INT_MAX));
+  p.chunk = q8_chunk((long long)max_blocks * bs);
   const int splits = q8_splits(max_ctx, window, p.chunk), blocks = q8_blocks(hd);
   const size_t row = (size_t)R * nh * splits;
   if (splits > 1) {
@@ -694,11 +723,14 @@ int zk_attention_q8(const void* q, int q_stride, const void* kcodes, const void*
   p.c2 = softcap * log2e;
   const int group = nh / nkv, tiles = (group + 15) / 16;
   const dim3 grid(splits, nkv * tiles, R);
+  // codes past the caches where one block alone reads them and the launch may pass through more than the memory side's cache holds
+  const bool once = tiles == 1 && (double)R * max_ctx * nkv * (2 * blocks * Q8_BLOCK + 8) > 256.0 * (1 << 20);
   const size_t lds = (size_t)4 * std::min(group, 16) * (blocks * Q8_BLOCK + 4) * sizeof(float);
+#define Q8_KERNEL(FMT, NB, CAP, DIRECT) (once ? attention_q8_kernel<FMT, NB, CAP, DIRECT, true> : attention_q8_kernel<FMT, NB, CAP, DIRECT, false>)
 #define Q8_ATTEND(FMT, NB)                                                                                             \
   do {                                                                                                                 \
-    const auto kernel = softcap > 0.f ? (splits > 1 ? attention_q8_kernel<FMT, NB, true, false> : attention_q8_kernel<FMT, NB, true, true>)    \
-                                      : (splits > 1 ? attention_q8_kernel<FMT, NB, false, false> : attention_q8_kernel<FMT, NB, false, true>); \
+    const auto kernel = softcap > 0.f ? (splits > 1 ? Q8_KERNEL(FMT, NB, true, false) : Q8_KERNEL(FMT, NB, true, true))    \
+                                      : (splits > 1 ? Q8_KERNEL(FMT, NB, false, false) : Q8_KERNEL(FMT, NB, false, true)); \
     if (lds > (64 << 10)) {                                                                                            \
       const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds); \
       if (e != hipSuccess) return zk_fail("zk_attention_q8: no room in LDS");                                          \
@@ -720,6 +752,7 @@ int zk_attention_q8(const void* q, int q_stride, const void* kcodes, const void*
   }
 #undef Q8_BY_BLOCKS
 #undef Q8_ATTEND
+#undef Q8_KERNEL
   return zk_launch_status("zk_attention_q8");
 }
 
