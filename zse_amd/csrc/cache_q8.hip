@@ -51,18 +51,6 @@ __device__ __forceinline__ unsigned q8_code(float x) {          // of a value ti
 #endif
   }
 }
-template <int FMT>
-__device__ __forceinline__ float q8_number(unsigned code) {
-  if constexpr (FMT == 0) return (float)(int)(int8_t)code;
-  else {
-#ifdef __HIP_DEVICE_COMPILE__
-    return __builtin_amdgcn_cvt_f32_fp8((int)code, 0);
-#else
-    return 0.f;
-#endif
-  }
-}
-
 // Scale and factor of a head whose largest magnitude is ``a`` (NaN or infinity where a value is not finite).
 template <int FMT>
 __device__ __forceinline__ void q8_scales(float a, float& scale, float& factor) {
@@ -80,135 +68,29 @@ __device__ __forceinline__ void q8_scales(float a, float& scale, float& factor) 
 // A value times its factor; 0 in a head whose scale says that nothing can be held.
 __device__ __forceinline__ float q8_times(float x, float factor) { return factor == 0.f ? 0.f : __fmul_rn(x, factor); }
 
-// The larger of two magnitudes, NaN if one is.
-__device__ __forceinline__ float q8_larger(float a, float b) { return a != a || b != b ? __int_as_float(0x7fc00000) : fmaxf(a, b); }
-
 // Sine and cosine of pos * freq, positions below 2^24.  The product is held in two floats (rounded to one it is off by up to half
-// a step of the angle, 2^-12 at position 4,096 and 2^-7 at 131,072), less whole turns (2 pi in two floats; n times the first
-// takes nothing from a multiple of its last place), then one float and what that leaves, which turns the result to first order.
+// a step of the angle, 2^-12 at position 4,096 and 2^-7 at 131,072), less whole quarters of a turn (pi / 2 in two floats; n times the
+// first takes nothing from a multiple of its last place), then one float r and what that leaves, which turns the result to first
+// order.  |r| is at most pi / 4 (and a rounding): the Taylor sums up to r^9 and r^10 are off by less than 2e-9.
 __device__ __forceinline__ void q8_sincos(float pos, float freq, float& sn, float& cs) {
   const float angle = __fmul_rn(pos, freq), low = __fmaf_rn(pos, freq, -angle);
-  const float n = rintf(angle * 0.15915494f);
-  const float a = __fmaf_rn(n, -6.2831855f, angle), b = __fmaf_rn(n, 1.7484556e-7f, low);
+  float n = rintf(angle * 0.63661977f);
+  float a = __fmaf_rn(n, -1.57079637f, angle), b = __fmaf_rn(n, 4.37113883e-8f, low);
+  n += rintf((a + b) * 0.63661977f);                 // (of large angles the first count is a quarter or two off)
+  a = __fmaf_rn(n, -1.57079637f, angle);
+  b = __fmaf_rn(n, 4.37113883e-8f, low);
   const float r = a + b, part = r - a, rest = (a - (r - part)) + (b - part);
-  float s, c;
-  sincosf(r, &s, &c);
-  sn = __fmaf_rn(c, rest, s);
-  cs = __fmaf_rn(s, -rest, c);
+  const float r2 = r * r, half = 0.5f * r2, one = 1.f - half;
+  const float s0 = __fmaf_rn(r * r2, __fmaf_rn(r2, __fmaf_rn(r2, __fmaf_rn(r2, 1.f / 362880.f, -1.f / 5040.f), 1.f / 120.f), -1.f / 6.f), r);
+  const float c4 = __fmaf_rn(r2, __fmaf_rn(r2, __fmaf_rn(r2, -1.f / 3628800.f, 1.f / 40320.f), -1.f / 720.f), 1.f / 24.f);
+  const float c0 = one + __fmaf_rn(r2 * r2, c4, (1.f - one) - half);
+  const float s = __fmaf_rn(c0, rest, s0), c = __fmaf_rn(s0, -rest, c0);
+  const int quarter = (int)n;
+  sn = quarter & 1 ? c : s;
+  cs = quarter & 1 ? s : c;
+  if (quarter & 2) sn = -sn;
+  if ((quarter + 1) & 2) cs = -cs;
 }
-
-// ---------------------------------------------------------------- written
-struct Q8Rows {
-  const act_t* rows;
-  const float* planes;        // partial sums of a split product, or none
-  int ld, sums;
-  size_t plane;
-  __device__ __forceinline__ float at(size_t t, int i) const {
-    if (sums <= 0) return to_f32(rows[t * ld + i]);
-    float x = planes[t * ld + i];
-    for (int p = 1; p < sums; p++) x += planes[p * plane + t * ld + i];
-    return to_f32(from_f32<act_t>(x));
-  }
-};
-
-template <int FMT>
-__global__ __launch_bounds__(64) void write_q8_kernel(Q8Rows from, act_t* q_out, int ldq, const int* __restrict__ positions,
-                                                      const int* __restrict__ slot_map, const float* __restrict__ inv_freq, int rotary_dim,
-                                                      uint8_t* __restrict__ kcodes, uint8_t* __restrict__ vcodes, float* __restrict__ scales,
-                                                      int nh, int nkv, int hd, int bs, int num_pages) {
-  const int t = blockIdx.x, head = blockIdx.y, lane = threadIdx.x, half = rotary_dim / 2;
-  const bool is_q = head < nh, is_v = head >= nh + nkv;
-  const int slot = slot_map && !is_q ? slot_map[t] : -1;
-  const bool store = slot >= 0 && slot / bs < num_pages;
-  if (!is_q && !store) return;
-  const float pos = (float)positions[t];
-  float x[4];
-#pragma unroll
-  for (int e = 0; e < 4; e++) {
-    const int c = lane + 64 * e;
-    x[e] = 0.f;
-    if (c >= hd) continue;
-    x[e] = from.at(t, head * hd + c);
-    if (!is_v && c < rotary_dim) {
-      const int i = c < half ? c : c - half;
-      const float other = from.at(t, head * hd + (c < half ? c + half : i));
-      float sn, cs, ra, rb;
-      q8_sincos(pos, inv_freq[i], sn, cs);
-      rotate_pair(c < half ? x[e] : other, c < half ? other : x[e], sn, cs, ra, rb);
-      x[e] = c < half ? ra : rb;
-    }
-  }
-  if (is_q) {
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-      if (lane + 64 * e < hd) q_out[(size_t)t * ldq + head * hd + lane + 64 * e] = from_f32<act_t>(x[e]);
-    return;
-  }
-  float a = 0.f;
-#pragma unroll
-  for (int e = 0; e < 4; e++) a = q8_larger(a, fabsf(x[e]));
-  const float bad = wave_max_whole(a != a ? 1.f : 0.f);
-  a = bad > 0.f ? __int_as_float(0x7fc00000) : wave_max_whole(a);
-  float scale, factor;
-  q8_scales<FMT>(a, scale, factor);
-  const int kvh = (head - nh) % nkv, page = slot / bs, off = slot % bs, blocks = q8_blocks(hd);
-  uint8_t* dst = (is_v ? vcodes : kcodes) + q8_piece(page, off / Q8_PIECE, kvh, nkv, bs / Q8_PIECE, blocks);
-#pragma unroll
-  for (int e = 0; e < 4; e++)
-    if (e < blocks)
-      dst[e * Q8_BYTES + (is_v ? q8_value_at(off % Q8_PIECE, lane) : q8_key_at(off % Q8_PIECE, lane))] =
-          (uint8_t)q8_code<FMT>(q8_times(x[e], factor));
-  if (lane == 0) scales[q8_scale(page, kvh, nkv, bs, is_v) + off] = scale;
-}
-
-// ---------------------------------------------------------------- read back
-template <int FMT>
-__global__ __launch_bounds__(256) void read_q8_kernel(const uint8_t* __restrict__ kcodes, const uint8_t* __restrict__ vcodes,
-                                                      const float* __restrict__ scales, const int* __restrict__ block_table, int max_blocks,
-                                                      const int* __restrict__ q_start, const int* __restrict__ ctx_len, act_t* __restrict__ k,
-                                                      act_t* __restrict__ v, int max_ctx, int window, int nkv, int hd, int bs, int num_pages,
-                                                      int v_transposed) {
-  const int j = blockIdx.x, head = blockIdx.y, r = blockIdx.z;
-  const int ctx = min(ctx_len[r], max_ctx);
-  const int rows = q_start ? q_start[r + 1] - q_start[r] : 1;
-  const int first = window > 0 ? max(0, ctx - rows + 1 - window) : 0;
-  if (j < first / bs || j * bs >= ctx) return;
-  const int page = block_table[(size_t)r * max_blocks + j];
-  if (page < 0 || page >= num_pages) return;
-  const int there = min(bs, ctx - j * bs), blocks = q8_blocks(hd);
-  const size_t out = ((size_t)page * nkv + head) * (size_t)(bs * hd);
-  for (int i = threadIdx.x; i < bs * hd; i += 256) {
-    const int t = i / hd, c = i % hd;
-    const size_t at = q8_piece(page, t / Q8_PIECE, head, nkv, bs / Q8_PIECE, blocks) + c / Q8_BLOCK * Q8_BYTES;
-    float x = 0.f, y = 0.f;
-    if (t < there) {
-      x = q8_number<FMT>(kcodes[at + q8_key_at(t % Q8_PIECE, c % Q8_BLOCK)]) * scales[q8_scale(page, head, nkv, bs, 0) + t];
-      y = q8_number<FMT>(vcodes[at + q8_value_at(t % Q8_PIECE, c % Q8_BLOCK)]) * scales[q8_scale(page, head, nkv, bs, 1) + t];
-    }
-    k[out + i] = from_f32<act_t>(x);
-    v[out + (v_transposed ? c * bs + t : i)] = from_f32<act_t>(y);
-  }
-}
-
-// ---------------------------------------------------------------- attended to
-// Scores and outputs by 16 x 16 matrix products whose columns are the query heads of one key head (16 at a time) and whose rows
-// are keys, then channels: S = K Q' over channels, O' = V' P over keys.  A lane of S holds four neighbouring keys of one head,
-// and that is the operand that O' takes: weights stay in registers.  Codes are whole in bfloat16 (8 bits of mantissa), so a
-// key's scale multiplies its score, a value's scale its weight.
-//
-// A block (four waves) takes a chunk of keys at absolute positions, a wave pairs of pieces of 16 in turn; the running maximum, the
-// sum and O' of the four waves are joined in LDS, the chunks' results by a second kernel.  The chunk follows from the width
-// of the table alone, so that a request's sums are cut alike whoever shares its step.
-struct Q8Attention {
-  const act_t* q;
-  const uint8_t *kcodes, *vcodes;
-  const float* scales;
-  const int *block_table, *ctx_len;
-  act_t* out;
-  float *part_o, *part_ml;          // [R][nh][splits][channels, filled up] and [..][2]
-  int q_stride, max_blocks, max_ctx, nh, nkv, hd, pieces, num_pages, window, chunk, q_whole;
-  float k1, k2, c2;                 // z log2(e) = k1 dot, or c2 tanh(k2 dot)
-};
 
 typedef float q8_f4 __attribute__((ext_vector_type(4)));
 typedef unsigned q8_u4 __attribute__((ext_vector_type(4)));
@@ -234,6 +116,280 @@ __device__ __forceinline__ void q8_floats(unsigned codes, float (&x)[4]) {
   }
 #endif
 }
+// ---------------------------------------------------------------- written
+// A block takes four rows of the step, a group of LANES lanes a head of them at a time, four neighbouring channels a lane: the
+// head's largest magnitude is a maximum over the group's lanes, and four rows whose slots are four in a row from a multiple of four on
+// (a portion) leave their values as whole words of the layout.  Sines and cosines of the block's rows are worked out once, in LDS.
+struct Q8Rows {
+  const act_t* rows;
+  const float* planes;        // partial sums of a split product, or none
+  int ld, sums;
+  size_t plane;
+  __device__ __forceinline__ float at(size_t i) const {
+    if (sums <= 0) return to_f32(rows[i]);
+    float x = planes[i];
+    for (int p = 1; p < sums; p++) x += planes[p * plane + i];
+    return to_f32(from_f32<act_t>(x));
+  }
+  __device__ __forceinline__ void at4(size_t i, float (&v)[4]) const {
+    typedef act_t a4 __attribute__((ext_vector_type(4)));
+    typedef float f4 __attribute__((ext_vector_type(4)));
+    if (sums <= 0) {
+      const a4 x = *(const a4*)(rows + i);
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[e] = to_f32(x[e]);
+      return;
+    }
+    f4 x = *(const f4*)(planes + i);
+    for (int p = 1; p < sums; p++) x += *(const f4*)(planes + p * plane + i);
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = to_f32(from_f32<act_t>(x[e]));
+  }
+};
+
+struct Q8Write {
+  Q8Rows from;
+  act_t* q_out;
+  const int *positions, *slot_map;
+  const float* inv_freq;
+  uint8_t *kcodes, *vcodes;
+  float* scales;
+  int ldq, rotary_dim, T, nh, nkv, hd, bs, num_pages, heads;
+};
+
+// The largest of a group of 16, 32 or 64 lanes' magnitudes as bits (a NaN is larger than infinity, and that than any number).
+template <int LANES>
+__device__ __forceinline__ float q8_largest(float v) {
+  auto larger = [](float a, float b) { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); };
+  float a = v, b = v;
+  if constexpr (LANES > 32) {
+    wave_pair32(v, a, b);
+    v = larger(a, b);
+  }
+  if constexpr (LANES > 16) {
+    wave_pair16(v, a, b);
+    v = larger(a, b);
+  }
+  v = larger(v, wave_dpp<ZSE_DPP_ROR8>(v));
+  v = larger(v, wave_dpp<ZSE_DPP_ROR4>(v));
+  v = larger(v, wave_dpp<ZSE_DPP_XOR2>(v));
+  return larger(v, wave_dpp<ZSE_DPP_XOR1>(v));
+}
+
+// WHOLE: rows, heads and half the rotation are whole fours at addresses of whole fours.
+template <int FMT, int LANES, bool WHOLE>
+__global__ __launch_bounds__(256) void write_q8_kernel(Q8Write p) {
+#ifdef __HIP_DEVICE_COMPILE__
+  constexpr int HEADS = 256 / LANES;                // of a pass
+  __shared__ float s_sin[4][128], s_cos[4][128];
+  const int t0 = blockIdx.x * 4, sub = threadIdx.x / LANES, c0 = threadIdx.x % LANES * 4, half = p.rotary_dim / 2;
+  const int blocks = q8_blocks(p.hd), pieces = p.bs / Q8_PIECE, n = min(4, p.T - t0);
+  int slot[4];
+#pragma unroll
+  for (int t = 0; t < 4; t++) {
+    slot[t] = p.slot_map && t < n ? p.slot_map[t0 + t] : -1;
+    if (slot[t] >= 0 && slot[t] / p.bs >= p.num_pages) slot[t] = -1;
+  }
+  const bool four = slot[0] >= 0 && slot[0] % 4 == 0 && slot[1] == slot[0] + 1 && slot[2] == slot[0] + 2 && slot[3] == slot[0] + 3;
+  const bool any = slot[0] >= 0 || slot[1] >= 0 || slot[2] >= 0 || slot[3] >= 0;
+  bool turned = false;
+  for (int base = blockIdx.y * HEADS; base < p.heads; base += gridDim.y * HEADS) {
+    const int head = min(base + sub, p.heads - 1);
+    const bool live = base + sub < p.heads, is_q = head < p.nh, is_v = head >= p.nh + p.nkv;
+    const bool turns = !is_v && c0 < p.rotary_dim;
+    float x[4][4], y[4][4];                         // a row's four channels, and those that they turn with
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[t][e] = y[t][e] = 0.f;
+      const size_t at = (size_t)(t0 + min(t, n - 1)) * p.from.ld + (size_t)head * p.hd;
+      if constexpr (WHOLE) {
+        if (c0 < p.hd) p.from.at4(at + c0, x[t]);
+        if (turns) p.from.at4(at + (c0 < half ? c0 + half : c0 - half), y[t]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int c = c0 + e;
+          if (c < p.hd) x[t][e] = p.from.at(at + c);
+          if (!is_v && c < p.rotary_dim) y[t][e] = p.from.at(at + (c < half ? c + half : c - half));
+        }
+      }
+    }
+    if (!turned && half > 0 && base < p.nh + p.nkv) {        // the block's first pass with queries or keys
+      for (int i = threadIdx.x; i < n * half; i += 256)
+        q8_sincos((float)p.positions[t0 + i / half], p.inv_freq[i % half], s_sin[i / half][i % half], s_cos[i / half][i % half]);
+      __syncthreads();
+      turned = true;
+    }
+    if (turns) {
+#pragma unroll
+      for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int c = c0 + e;
+          if (!WHOLE && c >= p.rotary_dim) continue;
+          const bool low = c < half;
+          const int tt = min(t, n - 1), i = low ? c : c - half;
+          float ra, rb;
+          rotate_pair(low ? x[t][e] : y[t][e], low ? y[t][e] : x[t][e], s_sin[tt][i], s_cos[tt][i], ra, rb);
+          x[t][e] = low ? ra : rb;
+        }
+    }
+    if (is_q && live) {
+#pragma unroll
+      for (int t = 0; t < 4; t++) {
+        if (t >= n) continue;
+        act_t* to = p.q_out + (size_t)(t0 + t) * p.ldq + (size_t)head * p.hd + c0;
+        if constexpr (WHOLE) {
+          typedef act_t a4 __attribute__((ext_vector_type(4)));
+          if (c0 < p.hd) *(a4*)to = a4{from_f32<act_t>(x[t][0]), from_f32<act_t>(x[t][1]), from_f32<act_t>(x[t][2]), from_f32<act_t>(x[t][3])};
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (c0 + e < p.hd) to[e] = from_f32<act_t>(x[t][e]);
+        }
+      }
+    }
+    if (!any || base + HEADS <= p.nh) continue;              // (all lanes of the block alike)
+    unsigned word[4];                                // a row's four codes
+    float scale[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+      float a = 0.f, factor;
+#pragma unroll
+      for (int e = 0; e < 4; e++) a = __uint_as_float(max(__float_as_uint(a), __float_as_uint(fabsf(x[t][e]))));
+      q8_scales<FMT>(q8_largest<LANES>(a), scale[t], factor);
+      word[t] = 0;
+#pragma unroll
+      for (int e = 0; e < 4; e++) word[t] |= q8_code<FMT>(q8_times(x[t][e], factor)) << (8 * e);
+    }
+    if (is_q || !live || c0 >= blocks * Q8_BLOCK) continue;
+    const int kvh = (head - p.nh) % p.nkv, j = c0 / Q8_BLOCK, c = c0 % Q8_BLOCK;
+    uint8_t* codes = (is_v ? p.vcodes : p.kcodes) + (size_t)j * Q8_BYTES;
+    auto piece = [&](int s) { return codes + q8_piece(s / p.bs, s % p.bs / Q8_PIECE, kvh, p.nkv, pieces, blocks); };
+    if (is_v && four) {
+      uint8_t* to = piece(slot[0]);
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        unsigned w = 0;
+#pragma unroll
+        for (int t = 0; t < 4; t++) w |= (word[t] >> (8 * e) & 255u) << (8 * t);
+        *(unsigned*)(to + q8_value_at(slot[0] % Q8_PIECE, c + e)) = w;
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < 4; t++) {
+        if (slot[t] < 0) continue;
+        uint8_t* to = piece(slot[t]);
+        if (is_v) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) to[q8_value_at(slot[t] % Q8_PIECE, c + e)] = (uint8_t)(word[t] >> (8 * e));
+        } else *(unsigned*)(to + q8_key_at(slot[t] % Q8_PIECE, c)) = word[t];
+      }
+    }
+    if (c0 == 0) {
+#pragma unroll
+      for (int t = 0; t < 4; t++)
+        if (slot[t] >= 0) p.scales[q8_scale(slot[t] / p.bs, kvh, p.nkv, p.bs, is_v) + slot[t] % p.bs] = scale[t];
+    }
+  }
+#endif
+}
+
+// ---------------------------------------------------------------- read back
+// A wave reads a piece of one head: keys eight channels a lane, so that a load is 512 bytes in a row and a store whole rows of 64
+// channels; values as the layout has them, four neighbouring tokens of four channels a lane.
+struct Q8Read {
+  const uint8_t *kcodes, *vcodes;
+  const float* scales;
+  const int *block_table, *q_start, *ctx_len;
+  act_t *k, *v;
+  int max_blocks, max_ctx, window, nkv, hd, bs, num_pages;
+};
+
+template <int FMT, bool TRANSPOSED, bool WHOLE>
+__global__ __launch_bounds__(256) void read_q8_kernel(Q8Read p) {
+#ifdef __HIP_DEVICE_COMPILE__
+  typedef unsigned u2 __attribute__((ext_vector_type(2)));
+  typedef act_t a4 __attribute__((ext_vector_type(4)));
+  typedef act_t a8 __attribute__((ext_vector_type(8)));
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), head = blockIdx.y, r = blockIdx.z;
+  const int i = blockIdx.x * 4 + wave, pieces = p.bs / Q8_PIECE;            // the request's i-th piece
+  const int ctx = min(p.ctx_len[r], p.max_ctx), rows = p.q_start ? p.q_start[r + 1] - p.q_start[r] : 1;
+  const int first = p.window > 0 ? max(0, ctx - rows + 1 - p.window) : 0;
+  if (i < first / p.bs * pieces || i / pieces * p.bs >= ctx) return;
+  const int page = p.block_table[(size_t)r * p.max_blocks + i / pieces];
+  if (page < 0 || page >= p.num_pages) return;
+  const int there = ctx - i * Q8_PIECE, blocks = q8_blocks(p.hd), sub = i % pieces;      // tokens that are there: below 1, none
+  const size_t at = q8_piece(page, sub, head, p.nkv, pieces, blocks);
+  const float* scales = p.scales + q8_scale(page, head, p.nkv, p.bs, 0) + sub * Q8_PIECE;
+  const size_t out = ((size_t)page * p.nkv + head) * (size_t)(p.bs * p.hd);
+  const int t0 = lane / 8, c8 = lane % 8 * 8;
+  const float ks[2] = {scales[t0], scales[t0 + 8]};
+  const q8_f4 vs = *(const q8_f4*)(scales + p.bs + lane / 16 * 4);
+  for (int j = 0; j < blocks; j++) {
+    u2 kw[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) kw[u] = *(const u2*)(p.kcodes + at + j * Q8_BYTES + u * 512 + lane * 8);
+    const q8_u4 vw = *(const q8_u4*)(p.vcodes + at + j * Q8_BYTES + lane * 16);
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const int t = t0 + 8 * u, c = j * Q8_BLOCK + c8;
+      float lo[4], hi[4];
+      q8_floats<FMT>(kw[u][0], lo);
+      q8_floats<FMT>(kw[u][1], hi);
+      a8 x;
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = from_f32<act_t>(t < there ? (e < 4 ? lo[e] : hi[e - 4]) * ks[u] : 0.f);
+      act_t* to = p.k + out + (size_t)(sub * Q8_PIECE + t) * p.hd + c;
+      if constexpr (WHOLE) {
+        if (c < p.hd) *(a8*)to = x;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (c + e < p.hd) to[e] = x[e];
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+      const int c = j * Q8_BLOCK + 16 * b + lane % 16, t = lane / 16 * 4;
+      float x[4];
+      q8_floats<FMT>(vw[b], x);
+      a4 y;
+#pragma unroll
+      for (int e = 0; e < 4; e++) y[e] = from_f32<act_t>(t + e < there ? x[e] * vs[e] : 0.f);
+      if (c < p.hd) {
+        if constexpr (TRANSPOSED) *(a4*)(p.v + out + (size_t)c * p.bs + sub * Q8_PIECE + t) = y;
+        else {
+#pragma unroll
+          for (int e = 0; e < 4; e++) p.v[out + (size_t)(sub * Q8_PIECE + t + e) * p.hd + c] = y[e];
+        }
+      }
+    }
+  }
+#endif
+}
+
+// ---------------------------------------------------------------- attended to
+// Scores and outputs by 16 x 16 matrix products whose columns are the query heads of one key head (16 at a time) and whose rows
+// are keys, then channels: S = K Q' over channels, O' = V' P over keys.  A lane of S holds four neighbouring keys of one head,
+// and that is the operand that O' takes: weights stay in registers.  Codes are whole in bfloat16 (8 bits of mantissa), so a
+// key's scale multiplies its score, a value's scale its weight.
+//
+// A block (four waves) takes a chunk of keys at absolute positions, a wave pairs of pieces of 16 in turn; the running maximum, the
+// sum and O' of the four waves are joined in LDS, the chunks' results by a second kernel.  The chunk follows from the width
+// of the table alone, so that a request's sums are cut alike whoever shares its step.
+struct Q8Attention {
+  const act_t* q;
+  const uint8_t *kcodes, *vcodes;
+  const float* scales;
+  const int *block_table, *ctx_len;
+  act_t* out;
+  float *part_o, *part_ml;          // [R][nh][splits][channels, filled up] and [..][2]
+  int q_stride, max_blocks, max_ctx, nh, nkv, hd, pieces, num_pages, window, chunk, q_whole;
+  float k1, k2, c2;                 // z log2(e) = k1 dot, or c2 tanh(k2 dot)
+};
+
 #if ZSE_ACT_BF16
 template <int FMT>
 __device__ __forceinline__ void q8_halves(unsigned codes, unsigned& lo, unsigned& hi) {
@@ -581,15 +737,9 @@ static int q8_refuses(const char* who, const void* kcodes, const void* vcodes, c
 }
 #define Q8_REQUIRE_CACHE(who) \
   if (const int rc = q8_refuses(who, kcodes, vcodes, scales, nkv, hd, bs, num_pages, format)) return rc
-#define Q8_FORMAT(call)            \
-  if (format == 0) {               \
-    constexpr int FMT = 0;         \
-    call;                          \
-  } else {                         \
-    constexpr int FMT = 1;         \
-    call;                          \
-  }
-
+#ifndef Q8_WRITE_BLOCKS
+#define Q8_WRITE_BLOCKS 1024
+#endif
 // Keys of a partial result, by what a request's table can hold.  us by 256, 512 and 1,024 keys (16-bit rows, 8 heads over 4 of 256
 // channels): one request of 4,000 keys 10.8, 12.8, 18.9; 64 of them 98.6, 93.7, 91.4; one of 16,000 15.6, 15.3, 20.8; eight of
 // them 56.3, 49.8, 47.9; one of 60,000 45.1, 33.5, 28.3.  32-bit products take eight times as long for as many keys: by 128, 256
@@ -634,11 +784,42 @@ int zk_rope_cache_write_q8(const void* qkv, int ld, const float* planes, int sum
   if (T == 0) return 0;
   ZK_REQUIRE(q_out && positions && (sums > 0 ? planes != nullptr && (uintptr_t)planes % 16 == 0 : qkv != nullptr),
              "zk_rope_cache_write_q8: null or misaligned argument");
-  const int width = (nh + 2 * nkv) * hd;
-  const Q8Rows from{(const act_t*)qkv, planes, sums > 0 ? width : ld, sums, (size_t)T * width};
-  Q8_FORMAT((write_q8_kernel<FMT><<<dim3(T, slot_map ? nh + 2 * nkv : nh), 64, 0, (hipStream_t)stream>>>(
-      from, (act_t*)q_out, ldq, positions, slot_map, inv_freq, rotary_dim, (uint8_t*)kcodes, (uint8_t*)vcodes, (float*)scales, nh, nkv, hd,
-      bs, num_pages)))
+  const int width = (nh + 2 * nkv) * hd, blocks = q8_blocks(hd);
+  Q8Write p;
+  p.from = Q8Rows{(const act_t*)qkv, planes, sums > 0 ? width : ld, sums, (size_t)T * width};
+  p.q_out = (act_t*)q_out;
+  p.positions = positions;
+  p.slot_map = slot_map;
+  p.inv_freq = inv_freq;
+  p.kcodes = (uint8_t*)kcodes;
+  p.vcodes = (uint8_t*)vcodes;
+  p.scales = (float*)scales;
+  p.ldq = ldq;
+  p.rotary_dim = rotary_dim;
+  p.T = T;
+  p.nh = nh;
+  p.nkv = nkv;
+  p.hd = hd;
+  p.bs = bs;
+  p.num_pages = num_pages;
+  p.heads = slot_map ? nh + 2 * nkv : nh;
+  const bool whole = hd % 4 == 0 && rotary_dim % 8 == 0 && p.from.ld % 4 == 0 && ldq % 4 == 0 && (uintptr_t)q_out % (4 * sizeof(act_t)) == 0 &&
+                     (sums > 0 || (uintptr_t)qkv % (4 * sizeof(act_t)) == 0);
+  const int lanes = blocks == 1 ? 16 : blocks == 2 ? 32 : 64, passes = (p.heads + 256 / lanes - 1) / (256 / lanes), groups = (T + 3) / 4;
+  const dim3 grid(groups, std::max(1, std::min(passes, Q8_WRITE_BLOCKS / groups)));
+#define Q8_WRITE_L(FMT, L) \
+  whole ? write_q8_kernel<FMT, L, true><<<grid, 256, 0, (hipStream_t)stream>>>(p) : write_q8_kernel<FMT, L, false><<<grid, 256, 0, (hipStream_t)stream>>>(p)
+#define Q8_WRITE(FMT)                            \
+  if (lanes == 16) Q8_WRITE_L(FMT, 16);          \
+  else if (lanes == 32) Q8_WRITE_L(FMT, 32);     \
+  else Q8_WRITE_L(FMT, 64);
+  if (format == 0) {
+    Q8_WRITE(0)
+  } else {
+    Q8_WRITE(1)
+  }
+#undef Q8_WRITE
+#undef Q8_WRITE_L
   return zk_launch_status("zk_rope_cache_write_q8");
 }
 
@@ -655,9 +836,35 @@ int zk_cache_read_q8(const void* kcodes, const void* vcodes, const float* scales
   ZK_REQUIRE(nkv <= 65535 && R <= 65535, "zk_cache_read_q8: too many requests or heads");
   if (R == 0 || max_ctx == 0) return 0;
   ZK_REQUIRE(block_table && ctx_len && k && v && ((uintptr_t)k | (uintptr_t)v) % 16 == 0, "zk_cache_read_q8: null or misaligned argument");
-  Q8_FORMAT((read_q8_kernel<FMT><<<dim3((max_ctx + bs - 1) / bs, nkv, R), 256, 0, (hipStream_t)stream>>>(
-      (const uint8_t*)kcodes, (const uint8_t*)vcodes, scales, block_table, max_blocks, q_start, ctx_len, (act_t*)k, (act_t*)v, max_ctx,
-      window, nkv, hd, bs, num_pages, v_transposed)))
+  Q8Read p;
+  p.kcodes = (const uint8_t*)kcodes;
+  p.vcodes = (const uint8_t*)vcodes;
+  p.scales = scales;
+  p.block_table = block_table;
+  p.q_start = q_start;
+  p.ctx_len = ctx_len;
+  p.k = (act_t*)k;
+  p.v = (act_t*)v;
+  p.max_blocks = max_blocks;
+  p.max_ctx = max_ctx;
+  p.window = window;
+  p.nkv = nkv;
+  p.hd = hd;
+  p.bs = bs;
+  p.num_pages = num_pages;
+  const int pieces = (max_ctx + bs - 1) / bs * (bs / Q8_PIECE);       // of whole pages
+  const dim3 grid((pieces + 3) / 4, nkv, R);
+  const bool whole = hd % 8 == 0;
+#define Q8_READ(FMT)                                                                                                  \
+  const auto kernel = v_transposed ? (whole ? read_q8_kernel<FMT, true, true> : read_q8_kernel<FMT, true, false>)     \
+                                   : (whole ? read_q8_kernel<FMT, false, true> : read_q8_kernel<FMT, false, false>);  \
+  kernel<<<grid, 256, 0, (hipStream_t)stream>>>(p);
+  if (format == 0) {
+    Q8_READ(0)
+  } else {
+    Q8_READ(1)
+  }
+#undef Q8_READ
   return zk_launch_status("zk_cache_read_q8");
 }
 
