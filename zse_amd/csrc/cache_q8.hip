@@ -16,6 +16,7 @@
 
 #include <algorithm>
 #include <cfloat>
+#include <type_traits>
 
 extern "C" int zk_steplist_register(const char* name, int nargs, void* fn);
 #define ZK_ENTER(fn) \
@@ -39,18 +40,26 @@ __device__ __forceinline__ size_t q8_scale(int page, int head, int nkv, int bs, 
 
 template <int FMT>
 __device__ __forceinline__ float q8_top() { return FMT == 0 ? 127.f : 448.f; }
+// Four values times ``factor`` as four codes.  |x| factor is at most top and a rounding, which the nearest code of either kind is top
+// for: nothing has to be cut off.
 template <int FMT>
-__device__ __forceinline__ unsigned q8_code(float x) {          // of a value times top / a
-  if constexpr (FMT == 0) return (unsigned)(int)fminf(fmaxf(rintf(x), -127.f), 127.f) & 255u;
-  else {
-    x = fminf(fmaxf(x, -448.f), 448.f);
+__device__ __forceinline__ unsigned q8_codes(const float (&x)[4], float factor) {
 #ifdef __HIP_DEVICE_COMPILE__
-    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false) & 255u;
-#else
-    return 0;
-#endif
+  if constexpr (FMT == 0) {
+    unsigned w[4];                    // 1.5 * 2^23 + a whole number: its two's complement in the lowest byte
+#pragma unroll
+    for (int e = 0; e < 4; e++) w[e] = __float_as_uint(__fmaf_rn(x[e], factor, 12582912.f));
+    const unsigned lo = __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0400), hi = __builtin_amdgcn_perm(w[3], w[2], 0x04000c0c);
+    return lo | hi;
+  } else {
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * factor, x[1] * factor, 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(x[2] * factor, x[3] * factor, lo, true);
   }
+#else
+  return 0;
+#endif
 }
+
 // Scale and factor of a head whose largest magnitude is ``a`` (NaN or infinity where a value is not finite).
 template <int FMT>
 __device__ __forceinline__ void q8_scales(float a, float& scale, float& factor) {
@@ -61,13 +70,10 @@ __device__ __forceinline__ void q8_scales(float a, float& scale, float& factor) 
   } else if (a < 0x1p-100f) {
     scale = factor = 0.f;
   } else {
-    scale = __fdiv_rn(a, top);
+    scale = __fmul_rn(a, 1.f / top);
     factor = __fdiv_rn(top, a);
   }
 }
-// A value times its factor; 0 in a head whose scale says that nothing can be held.
-__device__ __forceinline__ float q8_times(float x, float factor) { return factor == 0.f ? 0.f : __fmul_rn(x, factor); }
-
 // Sine and cosine of pos * freq, positions below 2^24.  The product is held in two floats (rounded to one it is off by up to half
 // a step of the angle, 2^-12 at position 4,096 and 2^-7 at 131,072), less whole quarters of a turn (pi / 2 in two floats; n times the
 // first takes nothing from a multiple of its last place), then one float r and what that leaves, which turns the result to first
@@ -119,36 +125,38 @@ __device__ __forceinline__ void q8_floats(unsigned codes, float (&x)[4]) {
 // ---------------------------------------------------------------- written
 // A block takes four rows of the step, a group of LANES lanes a head of them at a time, four neighbouring channels a lane: the
 // head's largest magnitude is a maximum over the group's lanes, and four rows whose slots are four in a row from a multiple of four on
-// (a portion) leave their values as whole words of the layout.  Sines and cosines of the block's rows are worked out once, in LDS.
+// (a portion's) leave their values as whole words of the layout.  Such fours are taken together wherever they begin; the rows that
+// are in none (single tokens, a portion's ends) are taken as they come.  Sines and cosines of the four rows are worked out once, in LDS.
+template <bool SUMS>
 struct Q8Rows {
   const act_t* rows;
-  const float* planes;        // partial sums of a split product, or none
+  const float* planes;        // partial sums of a split product
   int ld, sums;
   size_t plane;
   __device__ __forceinline__ float at(size_t i) const {
-    if (sums <= 0) return to_f32(rows[i]);
+    if constexpr (!SUMS) return to_f32(rows[i]);
     float x = planes[i];
     for (int p = 1; p < sums; p++) x += planes[p * plane + i];
     return to_f32(from_f32<act_t>(x));
   }
   __device__ __forceinline__ void at4(size_t i, float (&v)[4]) const {
     typedef act_t a4 __attribute__((ext_vector_type(4)));
-    typedef float f4 __attribute__((ext_vector_type(4)));
-    if (sums <= 0) {
+    if constexpr (!SUMS) {
       const a4 x = *(const a4*)(rows + i);
 #pragma unroll
       for (int e = 0; e < 4; e++) v[e] = to_f32(x[e]);
-      return;
-    }
-    f4 x = *(const f4*)(planes + i);
-    for (int p = 1; p < sums; p++) x += *(const f4*)(planes + p * plane + i);
+    } else {
+      q8_f4 x = *(const q8_f4*)(planes + i);
+      for (int p = 1; p < sums; p++) x += *(const q8_f4*)(planes + p * plane + i);
 #pragma unroll
-    for (int e = 0; e < 4; e++) v[e] = to_f32(from_f32<act_t>(x[e]));
+      for (int e = 0; e < 4; e++) v[e] = to_f32(from_f32<act_t>(x[e]));
+    }
   }
 };
 
+template <bool SUMS>
 struct Q8Write {
-  Q8Rows from;
+  Q8Rows<SUMS> from;
   act_t* q_out;
   const int *positions, *slot_map;
   const float* inv_freq;
@@ -177,120 +185,172 @@ __device__ __forceinline__ float q8_largest(float v) {
 }
 
 // WHOLE: rows, heads and half the rotation are whole fours at addresses of whole fours.
-template <int FMT, int LANES, bool WHOLE>
-__global__ __launch_bounds__(256) void write_q8_kernel(Q8Write p) {
+template <int FMT, int LANES, bool WHOLE, bool SUMS>
+__global__ __launch_bounds__(256, WHOLE ? 4 : 2) void write_q8_kernel(Q8Write<SUMS> p) {
 #ifdef __HIP_DEVICE_COMPILE__
   constexpr int HEADS = 256 / LANES;                // of a pass
-  __shared__ float s_sin[4][128], s_cos[4][128];
-  const int t0 = blockIdx.x * 4, sub = threadIdx.x / LANES, c0 = threadIdx.x % LANES * 4, half = p.rotary_dim / 2;
-  const int blocks = q8_blocks(p.hd), pieces = p.bs / Q8_PIECE, n = min(4, p.T - t0);
-  int slot[4];
-#pragma unroll
-  for (int t = 0; t < 4; t++) {
-    slot[t] = p.slot_map && t < n ? p.slot_map[t0 + t] : -1;
-    if (slot[t] >= 0 && slot[t] / p.bs >= p.num_pages) slot[t] = -1;
-  }
-  const bool four = slot[0] >= 0 && slot[0] % 4 == 0 && slot[1] == slot[0] + 1 && slot[2] == slot[0] + 2 && slot[3] == slot[0] + 3;
-  const bool any = slot[0] >= 0 || slot[1] >= 0 || slot[2] >= 0 || slot[3] >= 0;
-  bool turned = false;
-  for (int base = blockIdx.y * HEADS; base < p.heads; base += gridDim.y * HEADS) {
-    const int head = min(base + sub, p.heads - 1);
-    const bool live = base + sub < p.heads, is_q = head < p.nh, is_v = head >= p.nh + p.nkv;
-    const bool turns = !is_v && c0 < p.rotary_dim;
-    float x[4][4], y[4][4];                         // a row's four channels, and those that they turn with
+  __shared__ q8_f4 s_sin[4][32], s_cos[4][32];
+  const int lane = threadIdx.x & 63, sub = threadIdx.x / LANES, c0 = threadIdx.x % LANES * 4, half = p.rotary_dim / 2;
+  const int blocks = q8_blocks(p.hd), pieces = p.bs / Q8_PIECE, t0 = blockIdx.x * 4;
+  const bool rotated = c0 < p.rotary_dim, low = c0 < half, padded = c0 >= blocks * Q8_BLOCK;
+  // where a lane's channels, and those that they turn with, lie in a head; lanes without any read the head's first
+  const int own = c0 < p.hd ? c0 : 0, other = !rotated ? own : low ? c0 + half : c0 - half;
+  const int turn_at = rotated ? (low ? c0 : c0 - half) / 4 : 0;
+  const int key_at = c0 / Q8_BLOCK * Q8_BYTES + c0 % Q8_BLOCK, value_at = c0 / Q8_BLOCK * Q8_BYTES + q8_value_at(0, c0 % Q8_BLOCK);
+  const size_t head_bytes = (size_t)pieces * blocks * Q8_BYTES;
+  // lane i: the slot of row t0 - 3 + i, for ten rows; bit i of ``fours``: rows i to i + 3 are such a four
+  const int near = t0 - 3 + lane;
+  int slots = p.slot_map && lane < 10 && near >= 0 && near < p.T ? p.slot_map[near] : -1;
+  if (slots >= 0 && slots / p.bs >= p.num_pages) slots = -1;
+  const int s1 = __shfl(slots, lane + 1), s2 = __shfl(slots, lane + 2), s3 = __shfl(slots, lane + 3);
+  const unsigned fours = (unsigned)__ballot(lane < 7 && slots >= 0 && slots % 4 == 0 && s1 == slots + 1 && s2 == slots + 2 && s3 == slots + 3);
+  const int page = slots >= 0 ? slots / p.bs : 0, off = slots >= 0 ? slots % p.bs : 0;
+  for (int taken = 0; taken < 2; taken++) {
+    // the four that begins among the block's rows, then the block's rows that are in none
+    const bool four = taken == 0;
+    unsigned mine = 0;                                   // bit t: there is a row t
+    if (four) mine = fours & 0x78 ? 15 : 0;
+    else
+      for (int t = 0; t < 4; t++) mine |= !(fours >> t & 15) && t0 + t < p.T ? 1u << t : 0u;
+    if (!mine) continue;
+    const int start = four ? __builtin_ctz(fours & 0x78) : 3, present = start + __builtin_ctz(mine);
+    int row[4], slot[4], at[4];                          // what is not there is read as a row that is, and not stored
+    size_t piece[4], scale_at[4];
 #pragma unroll
     for (int t = 0; t < 4; t++) {
-#pragma unroll
-      for (int e = 0; e < 4; e++) x[t][e] = y[t][e] = 0.f;
-      const size_t at = (size_t)(t0 + min(t, n - 1)) * p.from.ld + (size_t)head * p.hd;
-      if constexpr (WHOLE) {
-        if (c0 < p.hd) p.from.at4(at + c0, x[t]);
-        if (turns) p.from.at4(at + (c0 < half ? c0 + half : c0 - half), y[t]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const int c = c0 + e;
-          if (c < p.hd) x[t][e] = p.from.at(at + c);
-          if (!is_v && c < p.rotary_dim) y[t][e] = p.from.at(at + (c < half ? c + half : c - half));
-        }
-      }
+      const int i = mine >> t & 1 ? start + t : present;
+      row[t] = t0 - 3 + i;
+      slot[t] = mine >> t & 1 ? __builtin_amdgcn_readlane(slots, i) : -1;
+      const int pg = __builtin_amdgcn_readlane(page, i), o = __builtin_amdgcn_readlane(off, i);
+      at[t] = o % Q8_PIECE;
+      piece[t] = ((size_t)pg * p.nkv * pieces + o / Q8_PIECE) * (size_t)(blocks * Q8_BYTES);
+      scale_at[t] = (size_t)pg * p.nkv * 2 * p.bs + o;
     }
-    if (!turned && half > 0 && base < p.nh + p.nkv) {        // the block's first pass with queries or keys
-      for (int i = threadIdx.x; i < n * half; i += 256)
-        q8_sincos((float)p.positions[t0 + i / half], p.inv_freq[i % half], s_sin[i / half][i % half], s_cos[i / half][i % half]);
-      __syncthreads();
-      turned = true;
-    }
-    if (turns) {
-#pragma unroll
-      for (int t = 0; t < 4; t++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const int c = c0 + e;
-          if (!WHOLE && c >= p.rotary_dim) continue;
-          const bool low = c < half;
-          const int tt = min(t, n - 1), i = low ? c : c - half;
-          float ra, rb;
-          rotate_pair(low ? x[t][e] : y[t][e], low ? y[t][e] : x[t][e], s_sin[tt][i], s_cos[tt][i], ra, rb);
-          x[t][e] = low ? ra : rb;
-        }
-    }
-    if (is_q && live) {
+    const bool stores = slot[0] >= 0 || slot[1] >= 0 || slot[2] >= 0 || slot[3] >= 0;
+    bool turned = false;
+    for (int base = blockIdx.y * HEADS; base < p.heads; base += gridDim.y * HEADS) {
+      const int head = min(base + sub, p.heads - 1);
+      const bool live = base + sub < p.heads, is_q = head < p.nh, is_v = head >= p.nh + p.nkv;
+      float x[4][4], y[4][4];                         // a row's four channels, and those that they turn with
 #pragma unroll
       for (int t = 0; t < 4; t++) {
-        if (t >= n) continue;
-        act_t* to = p.q_out + (size_t)(t0 + t) * p.ldq + (size_t)head * p.hd + c0;
+        const size_t from = (size_t)row[t] * p.from.ld + (size_t)head * p.hd;
         if constexpr (WHOLE) {
-          typedef act_t a4 __attribute__((ext_vector_type(4)));
-          if (c0 < p.hd) *(a4*)to = a4{from_f32<act_t>(x[t][0]), from_f32<act_t>(x[t][1]), from_f32<act_t>(x[t][2]), from_f32<act_t>(x[t][3])};
+          p.from.at4(from + own, x[t]);
+          p.from.at4(from + other, y[t]);
         } else {
 #pragma unroll
-          for (int e = 0; e < 4; e++)
-            if (c0 + e < p.hd) to[e] = from_f32<act_t>(x[t][e]);
+          for (int e = 0; e < 4; e++) {
+            const int c = c0 + e, mate = c >= p.rotary_dim ? c : c < half ? c + half : c - half;
+            x[t][e] = p.from.at(from + (c < p.hd ? c : 0));
+            y[t][e] = p.from.at(from + (c < p.hd ? mate : 0));
+          }
         }
       }
-    }
-    if (!any || base + HEADS <= p.nh) continue;              // (all lanes of the block alike)
-    unsigned word[4];                                // a row's four codes
-    float scale[4];
-#pragma unroll
-    for (int t = 0; t < 4; t++) {
-      float a = 0.f, factor;
-#pragma unroll
-      for (int e = 0; e < 4; e++) a = __uint_as_float(max(__float_as_uint(a), __float_as_uint(fabsf(x[t][e]))));
-      q8_scales<FMT>(q8_largest<LANES>(a), scale[t], factor);
-      word[t] = 0;
-#pragma unroll
-      for (int e = 0; e < 4; e++) word[t] |= q8_code<FMT>(q8_times(x[t][e], factor)) << (8 * e);
-    }
-    if (is_q || !live || c0 >= blocks * Q8_BLOCK) continue;
-    const int kvh = (head - p.nh) % p.nkv, j = c0 / Q8_BLOCK, c = c0 % Q8_BLOCK;
-    uint8_t* codes = (is_v ? p.vcodes : p.kcodes) + (size_t)j * Q8_BYTES;
-    auto piece = [&](int s) { return codes + q8_piece(s / p.bs, s % p.bs / Q8_PIECE, kvh, p.nkv, pieces, blocks); };
-    if (is_v && four) {
-      uint8_t* to = piece(slot[0]);
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        unsigned w = 0;
-#pragma unroll
-        for (int t = 0; t < 4; t++) w |= (word[t] >> (8 * e) & 255u) << (8 * t);
-        *(unsigned*)(to + q8_value_at(slot[0] % Q8_PIECE, c + e)) = w;
+      if (!turned && half > 0 && base < p.nh + p.nkv) {        // the first pass with queries or keys
+        if (taken) __syncthreads();                            // (the other rows' angles have been read)
+        for (int t = 0; t < 4; t++)
+          if (mine >> t & 1) {
+            const float pos = (float)p.positions[t == 0 ? row[0] : t == 1 ? row[1] : t == 2 ? row[2] : row[3]];
+            // a row a wave, so that all four are worked out side by side
+            if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) == t)
+              for (int i = lane; i < half; i += 64) q8_sincos(pos, p.inv_freq[i], ((float*)s_sin[t])[i], ((float*)s_cos[t])[i]);
+          }
+        __syncthreads();
+        turned = true;
       }
-    } else {
+      if (!is_v) {
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+          if constexpr (WHOLE) {
+            if (rotated) {
+              const q8_f4 sn = s_sin[t][turn_at], cs = s_cos[t][turn_at];
+#pragma unroll
+              for (int e = 0; e < 4; e++) x[t][e] = __fmaf_rn(x[t][e], cs[e], __fmul_rn(y[t][e], low ? -sn[e] : sn[e]));     // as rotate_pair
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const int c = c0 + e;
+              if (c >= p.rotary_dim) continue;
+              const bool first = c < half;
+              const int i = first ? c : c - half;
+              const float sn = ((const float*)s_sin[t])[i], cs = ((const float*)s_cos[t])[i];
+              x[t][e] = __fmaf_rn(x[t][e], cs, __fmul_rn(y[t][e], first ? -sn : sn));
+            }
+          }
+        }
+      }
+      if (is_q && live) {
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+          if (!(mine >> t & 1)) continue;
+          act_t* to = p.q_out + (size_t)row[t] * p.ldq + (size_t)head * p.hd + c0;
+          if constexpr (WHOLE) {
+            typedef act_t a4 __attribute__((ext_vector_type(4)));
+            if (c0 < p.hd) *(a4*)to = a4{from_f32<act_t>(x[t][0]), from_f32<act_t>(x[t][1]), from_f32<act_t>(x[t][2]), from_f32<act_t>(x[t][3])};
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              if (c0 + e < p.hd) to[e] = from_f32<act_t>(x[t][e]);
+          }
+        }
+      }
+      if (!stores || base + HEADS <= p.nh) continue;           // (all lanes of the block alike)
+      float most[4];
 #pragma unroll
       for (int t = 0; t < 4; t++) {
-        if (slot[t] < 0) continue;
-        uint8_t* to = piece(slot[t]);
-        if (is_v) {
+        unsigned a = 0;
 #pragma unroll
-          for (int e = 0; e < 4; e++) to[q8_value_at(slot[t] % Q8_PIECE, c + e)] = (uint8_t)(word[t] >> (8 * e));
-        } else *(unsigned*)(to + q8_key_at(slot[t] % Q8_PIECE, c)) = word[t];
+        for (int e = 0; e < 4; e++) {
+          if (c0 + e >= p.hd) x[t][e] = 0.f;                   // the last block is filled up with zeros
+          a = max(a, __float_as_uint(x[t][e]) & 0x7fffffffu);
+        }
+        most[t] = q8_largest<LANES>(__uint_as_float(a));
       }
-    }
-    if (c0 == 0) {
+      // a lane works out one row's factor for the four lanes of its quad
+      float scale, factor;
+      q8_scales<FMT>(lane & 2 ? (lane & 1 ? most[3] : most[2]) : (lane & 1 ? most[1] : most[0]), scale, factor);
+      const float factors[4] = {wave_dpp<0x00>(factor), wave_dpp<0x55>(factor), wave_dpp<0xAA>(factor), wave_dpp<0xFF>(factor)};
+      unsigned word[4];                                // a row's four codes
 #pragma unroll
-      for (int t = 0; t < 4; t++)
-        if (slot[t] >= 0) p.scales[q8_scale(slot[t] / p.bs, kvh, p.nkv, p.bs, is_v) + slot[t] % p.bs] = scale[t];
+      for (int t = 0; t < 4; t++) {
+        if (factors[t] == 0.f) {                       // nothing that a code could hold, or a value that is not finite
+#pragma unroll
+          for (int e = 0; e < 4; e++) x[t][e] = 0.f;
+        }
+        word[t] = q8_codes<FMT>(x[t], factors[t]);
+      }
+      if (is_q || !live) continue;
+      const int kvh = (head - p.nh) - (is_v ? p.nkv : 0);
+      uint8_t* codes = (is_v ? p.vcodes : p.kcodes) + kvh * head_bytes;
+      if (!padded) {
+        if (is_v && four) {
+          // the four rows' bytes of a channel side by side
+          const unsigned a = __builtin_amdgcn_perm(word[1], word[0], 0x05010400), b = __builtin_amdgcn_perm(word[1], word[0], 0x07030602);
+          const unsigned d = __builtin_amdgcn_perm(word[3], word[2], 0x05010400), f = __builtin_amdgcn_perm(word[3], word[2], 0x07030602);
+          unsigned* to = (unsigned*)(codes + piece[0] + value_at + at[0] * 64);      // (the next channel: 16 bytes on)
+          to[0] = __builtin_amdgcn_perm(d, a, 0x05040100);
+          to[4] = __builtin_amdgcn_perm(d, a, 0x07060302);
+          to[8] = __builtin_amdgcn_perm(f, b, 0x05040100);
+          to[12] = __builtin_amdgcn_perm(f, b, 0x07060302);
+        } else {
+#pragma unroll
+          for (int t = 0; t < 4; t++) {
+            if (slot[t] < 0) continue;
+            if (is_v) {
+              uint8_t* to = codes + piece[t] + value_at + at[t] / 4 * 256 + at[t] % 4;
+#pragma unroll
+              for (int e = 0; e < 4; e++) to[16 * e] = (uint8_t)(word[t] >> (8 * e));
+            } else *(unsigned*)(codes + piece[t] + key_at + at[t] * 64) = word[t];
+          }
+        }
+      }
+      if (c0 < 16) {                                   // the head's first four lanes: a row's scale each
+        const int t = lane & 3;
+        const size_t to = t == 0 ? scale_at[0] : t == 1 ? scale_at[1] : t == 2 ? scale_at[2] : scale_at[3];
+        if ((t == 0 ? slot[0] : t == 1 ? slot[1] : t == 2 ? slot[2] : slot[3]) >= 0) p.scales[to + (size_t)(2 * kvh + is_v) * p.bs] = scale;
+      }
     }
   }
 #endif
@@ -304,7 +364,7 @@ struct Q8Read {
   const float* scales;
   const int *block_table, *q_start, *ctx_len;
   act_t *k, *v;
-  int max_blocks, max_ctx, window, nkv, hd, bs, num_pages;
+  int R, max_blocks, max_ctx, window, nkv, hd, bs, num_pages;
 };
 
 template <int FMT, bool TRANSPOSED, bool WHOLE>
@@ -313,56 +373,70 @@ __global__ __launch_bounds__(256) void read_q8_kernel(Q8Read p) {
   typedef unsigned u2 __attribute__((ext_vector_type(2)));
   typedef act_t a4 __attribute__((ext_vector_type(4)));
   typedef act_t a8 __attribute__((ext_vector_type(8)));
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), head = blockIdx.y, r = blockIdx.z;
-  const int i = blockIdx.x * 4 + wave, pieces = p.bs / Q8_PIECE;            // the request's i-th piece
-  const int ctx = min(p.ctx_len[r], p.max_ctx), rows = p.q_start ? p.q_start[r + 1] - p.q_start[r] : 1;
-  const int first = p.window > 0 ? max(0, ctx - rows + 1 - p.window) : 0;
-  if (i < first / p.bs * pieces || i / pieces * p.bs >= ctx) return;
-  const int page = p.block_table[(size_t)r * p.max_blocks + i / pieces];
-  if (page < 0 || page >= p.num_pages) return;
-  const int there = ctx - i * Q8_PIECE, blocks = q8_blocks(p.hd), sub = i % pieces;      // tokens that are there: below 1, none
-  const size_t at = q8_piece(page, sub, head, p.nkv, pieces, blocks);
-  const float* scales = p.scales + q8_scale(page, head, p.nkv, p.bs, 0) + sub * Q8_PIECE;
-  const size_t out = ((size_t)page * p.nkv + head) * (size_t)(p.bs * p.hd);
-  const int t0 = lane / 8, c8 = lane % 8 * 8;
-  const float ks[2] = {scales[t0], scales[t0 + 8]};
-  const q8_f4 vs = *(const q8_f4*)(scales + p.bs + lane / 16 * 4);
-  for (int j = 0; j < blocks; j++) {
-    u2 kw[2];
-#pragma unroll
-    for (int u = 0; u < 2; u++) kw[u] = *(const u2*)(p.kcodes + at + j * Q8_BYTES + u * 512 + lane * 8);
-    const q8_u4 vw = *(const q8_u4*)(p.vcodes + at + j * Q8_BYTES + lane * 16);
-#pragma unroll
-    for (int u = 0; u < 2; u++) {
-      const int t = t0 + 8 * u, c = j * Q8_BLOCK + c8;
-      float lo[4], hi[4];
-      q8_floats<FMT>(kw[u][0], lo);
-      q8_floats<FMT>(kw[u][1], hi);
-      a8 x;
-#pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = from_f32<act_t>(t < there ? (e < 4 ? lo[e] : hi[e - 4]) * ks[u] : 0.f);
-      act_t* to = p.k + out + (size_t)(sub * Q8_PIECE + t) * p.hd + c;
-      if constexpr (WHOLE) {
-        if (c < p.hd) *(a8*)to = x;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-          if (c + e < p.hd) to[e] = x[e];
-      }
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pieces = p.bs / Q8_PIECE, per_page = pieces * p.nkv;
+  // the requests' pages are numbered through, 64 requests at a time: lane i knows where those of request r0 + i end
+  int r0 = -64, before = 0, upto = 0, ends = 0, ctx_of = 0, first_of = 0;      // before, upto: of the 64 requests' pages
+  for (int item = blockIdx.x * 4 + wave;; item += gridDim.x * 4) {
+    const int x = item / per_page, rest = item % per_page, head = rest / pieces, sub = rest % pieces;
+    while (x >= upto) {
+      r0 += 64;
+      if (r0 >= p.R) return;
+      const int r = min(r0 + lane, p.R - 1), ctx = min(p.ctx_len[r], p.max_ctx), rows = p.q_start ? p.q_start[r + 1] - p.q_start[r] : 1;
+      ctx_of = ctx;
+      first_of = (p.window > 0 ? max(0, ctx - rows + 1 - p.window) : 0) / p.bs;
+      ends = upto + wave_running_sum(r0 + lane < p.R ? max(0, (ctx + p.bs - 1) / p.bs - first_of) : 0);
+      before = upto;
+      upto = __builtin_amdgcn_readlane(ends, 63);
     }
+    const int of = __ffsll(__ballot(ends > x)) - 1, r = r0 + of;
+    const int ctx = __builtin_amdgcn_readlane(ctx_of, of);
+    const int j = __builtin_amdgcn_readlane(first_of, of) + x - (of ? __builtin_amdgcn_readlane(ends, of - 1) : before);
+    const int page = p.block_table[(size_t)r * p.max_blocks + j], i = j * pieces + sub;
+    if (page < 0 || page >= p.num_pages) continue;
+    const int there = ctx - i * Q8_PIECE, blocks = q8_blocks(p.hd);      // tokens that are there: below 1, none
+    const size_t at = q8_piece(page, sub, head, p.nkv, pieces, blocks);
+    const float* scales = p.scales + q8_scale(page, head, p.nkv, p.bs, 0) + sub * Q8_PIECE;
+    const size_t out = ((size_t)page * p.nkv + head) * (size_t)(p.bs * p.hd);
+    const int t0 = lane / 8, c8 = lane % 8 * 8;
+    const float ks[2] = {scales[t0], scales[t0 + 8]};
+    const q8_f4 vs = *(const q8_f4*)(scales + p.bs + lane / 16 * 4);
+    for (int n = 0; n < blocks; n++) {
+      u2 kw[2];
 #pragma unroll
-    for (int b = 0; b < 4; b++) {
-      const int c = j * Q8_BLOCK + 16 * b + lane % 16, t = lane / 16 * 4;
-      float x[4];
-      q8_floats<FMT>(vw[b], x);
-      a4 y;
+      for (int u = 0; u < 2; u++) kw[u] = *(const u2*)(p.kcodes + at + n * Q8_BYTES + u * 512 + lane * 8);
+      const q8_u4 vw = *(const q8_u4*)(p.vcodes + at + n * Q8_BYTES + lane * 16);
 #pragma unroll
-      for (int e = 0; e < 4; e++) y[e] = from_f32<act_t>(t + e < there ? x[e] * vs[e] : 0.f);
-      if (c < p.hd) {
-        if constexpr (TRANSPOSED) *(a4*)(p.v + out + (size_t)c * p.bs + sub * Q8_PIECE + t) = y;
-        else {
+      for (int u = 0; u < 2; u++) {
+        const int t = t0 + 8 * u, c = n * Q8_BLOCK + c8;
+        float lo[4], hi[4];
+        q8_floats<FMT>(kw[u][0], lo);
+        q8_floats<FMT>(kw[u][1], hi);
+        a8 x;
 #pragma unroll
-          for (int e = 0; e < 4; e++) p.v[out + (size_t)(sub * Q8_PIECE + t + e) * p.hd + c] = y[e];
+        for (int e = 0; e < 8; e++) x[e] = from_f32<act_t>(t < there ? (e < 4 ? lo[e] : hi[e - 4]) * ks[u] : 0.f);
+        act_t* to = p.k + out + (size_t)(sub * Q8_PIECE + t) * p.hd + c;
+        if constexpr (WHOLE) {
+          if (c < p.hd) *(a8*)to = x;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; e++)
+            if (c + e < p.hd) to[e] = x[e];
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < 4; b++) {
+        const int c = n * Q8_BLOCK + 16 * b + lane % 16, t = lane / 16 * 4;
+        float x[4];
+        q8_floats<FMT>(vw[b], x);
+        a4 y;
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = from_f32<act_t>(t + e < there ? x[e] * vs[e] : 0.f);
+        if (c < p.hd) {
+          if constexpr (TRANSPOSED) *(a4*)(p.v + out + (size_t)c * p.bs + sub * Q8_PIECE + t) = y;
+          else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) p.v[out + (size_t)(sub * Q8_PIECE + t + e) * p.hd + c] = y[e];
+          }
         }
       }
     }
@@ -737,9 +811,24 @@ static int q8_refuses(const char* who, const void* kcodes, const void* vcodes, c
 }
 #define Q8_REQUIRE_CACHE(who) \
   if (const int rc = q8_refuses(who, kcodes, vcodes, scales, nkv, hd, bs, num_pages, format)) return rc
-#ifndef Q8_WRITE_BLOCKS
-#define Q8_WRITE_BLOCKS 1024
-#endif
+// Blocks of a launch.  Written: the heads of four rows are dealt to as many blocks as that gives (4,092 rows of 32 heads and 2 x 16 of
+// 128 channels by 1,024, 2,048 and 4,096 blocks 43, 40 and 38 us; more work out the same angles).  Read back: waves that take
+// pieces in turn (64 pages of 8 heads in a range of 64,512 pieces by 2,048, 4,096 and 8,192 blocks 6.2, 8.1 and 10.4 us, empty ones
+// cost as much as others; 147,000 pieces that are all there 56.9, 56.3 and 56.2).
+#define Q8_WRITE_BLOCKS 4096
+#define Q8_READ_BLOCKS 2048
+
+// Calls ``go`` with what is only known at run time as a constant.
+template <typename F>
+static void q8_by_format(int format, F go) {
+  if (format == 0) go(std::integral_constant<int, 0>());
+  else go(std::integral_constant<int, 1>());
+}
+template <typename F>
+static void q8_by_flag(bool flag, F go) {
+  if (flag) go(std::true_type());
+  else go(std::false_type());
+}
 // Keys of a partial result, by what a request's table can hold.  us by 256, 512 and 1,024 keys (16-bit rows, 8 heads over 4 of 256
 // channels): one request of 4,000 keys 10.8, 12.8, 18.9; 64 of them 98.6, 93.7, 91.4; one of 16,000 15.6, 15.3, 20.8; eight of
 // them 56.3, 49.8, 47.9; one of 60,000 45.1, 33.5, 28.3.  32-bit products take eight times as long for as many keys: by 128, 256
@@ -785,41 +874,28 @@ int zk_rope_cache_write_q8(const void* qkv, int ld, const float* planes, int sum
   ZK_REQUIRE(q_out && positions && (sums > 0 ? planes != nullptr && (uintptr_t)planes % 16 == 0 : qkv != nullptr),
              "zk_rope_cache_write_q8: null or misaligned argument");
   const int width = (nh + 2 * nkv) * hd, blocks = q8_blocks(hd);
-  Q8Write p;
-  p.from = Q8Rows{(const act_t*)qkv, planes, sums > 0 ? width : ld, sums, (size_t)T * width};
-  p.q_out = (act_t*)q_out;
-  p.positions = positions;
-  p.slot_map = slot_map;
-  p.inv_freq = inv_freq;
-  p.kcodes = (uint8_t*)kcodes;
-  p.vcodes = (uint8_t*)vcodes;
-  p.scales = (float*)scales;
-  p.ldq = ldq;
-  p.rotary_dim = rotary_dim;
-  p.T = T;
-  p.nh = nh;
-  p.nkv = nkv;
-  p.hd = hd;
-  p.bs = bs;
-  p.num_pages = num_pages;
-  p.heads = slot_map ? nh + 2 * nkv : nh;
-  const bool whole = hd % 4 == 0 && rotary_dim % 8 == 0 && p.from.ld % 4 == 0 && ldq % 4 == 0 && (uintptr_t)q_out % (4 * sizeof(act_t)) == 0 &&
-                     (sums > 0 || (uintptr_t)qkv % (4 * sizeof(act_t)) == 0);
-  const int lanes = blocks == 1 ? 16 : blocks == 2 ? 32 : 64, passes = (p.heads + 256 / lanes - 1) / (256 / lanes), groups = (T + 3) / 4;
+  const bool partial = sums > 0;
+  const int row = partial ? width : ld, heads = slot_map ? nh + 2 * nkv : nh;
+  const bool whole = hd % 4 == 0 && rotary_dim % 8 == 0 && row % 4 == 0 && ldq % 4 == 0 && (uintptr_t)q_out % (4 * sizeof(act_t)) == 0 &&
+                     (partial || (uintptr_t)qkv % (4 * sizeof(act_t)) == 0);
+  const int lanes = blocks == 1 ? 16 : blocks == 2 ? 32 : 64, passes = (heads + 256 / lanes - 1) / (256 / lanes), groups = (T + 3) / 4;
   const dim3 grid(groups, std::max(1, std::min(passes, Q8_WRITE_BLOCKS / groups)));
-#define Q8_WRITE_L(FMT, L) \
-  whole ? write_q8_kernel<FMT, L, true><<<grid, 256, 0, (hipStream_t)stream>>>(p) : write_q8_kernel<FMT, L, false><<<grid, 256, 0, (hipStream_t)stream>>>(p)
-#define Q8_WRITE(FMT)                            \
-  if (lanes == 16) Q8_WRITE_L(FMT, 16);          \
-  else if (lanes == 32) Q8_WRITE_L(FMT, 32);     \
-  else Q8_WRITE_L(FMT, 64);
-  if (format == 0) {
-    Q8_WRITE(0)
-  } else {
-    Q8_WRITE(1)
-  }
-#undef Q8_WRITE
-#undef Q8_WRITE_L
+  auto launch = [&](auto format_of, auto lanes_of, auto whole_of, auto partial_of) {
+    constexpr bool SUMS = decltype(partial_of)::value;
+    const Q8Write<SUMS> p{{(const act_t*)qkv, planes, row, sums, (size_t)T * width}, (act_t*)q_out, positions, slot_map, inv_freq,
+                          (uint8_t*)kcodes, (uint8_t*)vcodes, (float*)scales, ldq, rotary_dim, T, nh, nkv, hd, bs, num_pages, heads};
+    write_q8_kernel<decltype(format_of)::value, decltype(lanes_of)::value, decltype(whole_of)::value, SUMS>
+        <<<grid, 256, 0, (hipStream_t)stream>>>(p);
+  };
+  q8_by_format(format, [&](auto f) {
+    q8_by_flag(whole, [&](auto w) {
+      q8_by_flag(partial, [&](auto s) {
+        if (lanes == 16) launch(f, std::integral_constant<int, 16>(), w, s);
+        else if (lanes == 32) launch(f, std::integral_constant<int, 32>(), w, s);
+        else launch(f, std::integral_constant<int, 64>(), w, s);
+      });
+    });
+  });
   return zk_launch_status("zk_rope_cache_write_q8");
 }
 
@@ -852,19 +928,18 @@ int zk_cache_read_q8(const void* kcodes, const void* vcodes, const float* scales
   p.hd = hd;
   p.bs = bs;
   p.num_pages = num_pages;
-  const int pieces = (max_ctx + bs - 1) / bs * (bs / Q8_PIECE);       // of whole pages
-  const dim3 grid((pieces + 3) / 4, nkv, R);
-  const bool whole = hd % 8 == 0;
-#define Q8_READ(FMT)                                                                                                  \
-  const auto kernel = v_transposed ? (whole ? read_q8_kernel<FMT, true, true> : read_q8_kernel<FMT, true, false>)     \
-                                   : (whole ? read_q8_kernel<FMT, false, true> : read_q8_kernel<FMT, false, false>);  \
-  kernel<<<grid, 256, 0, (hipStream_t)stream>>>(p);
-  if (format == 0) {
-    Q8_READ(0)
-  } else {
-    Q8_READ(1)
-  }
-#undef Q8_READ
+  p.R = R;
+  // how much of it the requests' windows cover is not known here: blocks enough to fill the chip, whose waves take pieces in turn
+  const long long pieces = (long long)((max_ctx + bs - 1) / bs) * (bs / Q8_PIECE) * nkv * R;
+  ZK_REQUIRE(pieces < (1ll << 30), "zk_cache_read_q8: too many pages");
+  const int grid = (int)std::min<long long>((pieces + 3) / 4, Q8_READ_BLOCKS);
+  q8_by_format(format, [&](auto f) {
+    q8_by_flag(v_transposed != 0, [&](auto t) {
+      q8_by_flag(hd % 8 == 0, [&](auto w) {
+        read_q8_kernel<decltype(f)::value, decltype(t)::value, decltype(w)::value><<<grid, 256, 0, (hipStream_t)stream>>>(p);
+      });
+    });
+  });
   return zk_launch_status("zk_cache_read_q8");
 }
 
