@@ -105,3 +105,13 @@ def test_layout_is_one_to_one():
 def test_numbers():
     assert P.numbers(np.array([0x7e, 0xfe, 0x38, 0x01, 0x00], np.uint8), 1).tolist() == [448.0, -448.0, 1.0, 2.0 ** -9, 0.0]
     assert P.numbers(np.array([0x7f, 0x81, 0xff, 0], np.uint8), 0).tolist() == [127.0, -127.0, -1.0, 0.0]
+
+
+def test_names():
+    from zse_amd.runtime.device import canonical_cache_dtype
+    assert canonical_cache_dtype(None, "bfloat16") is None and canonical_cache_dtype("bf16", "bfloat16") is None
+    assert canonical_cache_dtype("float32", "fp32") is None
+    assert canonical_cache_dtype("INT8", "float32") == "int8" and canonical_cache_dtype("fp8", "bfloat16") == "float8_e4m3"
+    for bad in ("int4", "float32", ""):
+        with pytest.raises(ValueError, match="cache_dtype must be one of"):
+            canonical_cache_dtype(bad, "bfloat16")

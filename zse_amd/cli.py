@@ -45,7 +45,8 @@ def _cmd_generate(a):
         model = random_model(read_config_json(a.model), a.dtype, seed=a.weight_seed)
     eng = Engine(model, dtype=a.dtype, block_size=a.block_size, num_blocks=a.num_blocks,
                  max_batch_tokens=a.max_batch_tokens, max_batch_seqs=a.max_batch_seqs,
-                 prefill_chunk_size=a.prefill_chunk_size, max_seq_len=a.max_seq_len, quiet=a.quiet)
+                 prefill_chunk_size=a.prefill_chunk_size, max_seq_len=a.max_seq_len, quiet=a.quiet,
+                 cache_dtype=a.cache_dtype)
     sp = SamplingParams(max_tokens=a.max_tokens, temperature=a.temperature, top_p=a.top_p,
                         top_k=a.top_k, repetition_penalty=a.repetition_penalty,
                         stop_tokens=_ids(a.stop_tokens) if a.stop_tokens else None, seed=a.seed)
@@ -63,6 +64,8 @@ def _cmd_replay(a):
     from .engine.replay import main as replay_main
     argv = ["--model", a.model, "--dtype", a.dtype, "--out", a.out, "--max-tokens", str(a.max_tokens),
             "--block-size", str(a.block_size)]
+    if a.cache_dtype:
+        argv += ["--cache-dtype", a.cache_dtype]
     if a.trace:
         sys.stdin = open(a.trace)
     return replay_main(argv)
@@ -125,6 +128,8 @@ def main(argv=None):
     g.add_argument("--stop-tokens", help="token ids that end a request")
     g.add_argument("--seed", type=int, default=None)
     g.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "bf16", "float32", "fp32"])
+    g.add_argument("--cache-dtype", default=None, choices=["int8", "float8_e4m3"],
+                   help="hold cached keys and values in 8 bits (default: in the compute type)")
     g.add_argument("--block-size", type=int, default=16)
     g.add_argument("--num-blocks", type=int, default=None)
     g.add_argument("--max-batch-tokens", type=int, default=4096)
@@ -143,6 +148,7 @@ def main(argv=None):
     r.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
     r.add_argument("--max-tokens", type=int, required=True)
     r.add_argument("--block-size", type=int, default=16)
+    r.add_argument("--cache-dtype", default=None, choices=["int8", "float8_e4m3"])
 
     sub.add_parser("info", help="show the GPU")
     sub.add_parser("version", help="show the version")

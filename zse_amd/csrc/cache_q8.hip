@@ -677,15 +677,23 @@ __global__ __launch_bounds__(256, 2) void attention_q8_kernel(Q8Attention p) {
         w[u][i] = e * vs[u][i];
       }
 #if ZSE_ACT_BF16
-    // the weights round to the values' type (half a step of 2^-8 each); their sum does not
-    q8_b8 pb;
+    // A weight meets the values as two numbers, its rounded value and what the rounding left (16 bits of mantissa): with the first alone
+    // the results are 1.5 times as far from 64 bits (2.6e-3 of them instead of 1.7e-3, which is their own rounding), and the products
+    // are not what bounds the kernel.
+    q8_b8 pb, rest;
 #pragma unroll
-    for (int e = 0; e < 8; e++) pb[e] = (__bf16)w[e / 4][e % 4];
+    for (int e = 0; e < 8; e++) {
+      pb[e] = (__bf16)w[e / 4][e % 4];
+      rest[e] = (__bf16)(w[e / 4][e % 4] - (float)pb[e]);
+    }
 #pragma unroll
     for (int j = 0; j < NB; j++)
 #pragma unroll
-      for (int b = 0; b < 4; b++)
-        o[4 * j + b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q8_operand<FMT>(vc[0][j][b], vc[1][j][b]), pb, o[4 * j + b], 0, 0, 0);
+      for (int b = 0; b < 4; b++) {
+        const q8_b8 v = q8_operand<FMT>(vc[0][j][b], vc[1][j][b]);
+        o[4 * j + b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pb, o[4 * j + b], 0, 0, 0);
+        o[4 * j + b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, rest, o[4 * j + b], 0, 0, 0);
+      }
 #else
 #pragma unroll
     for (int u = 0; u < 2; u++)

@@ -15,7 +15,7 @@ from collections import deque
 from dataclasses import dataclass, field
 from typing import Dict, Iterator, List, Optional, Sequence, Union
 
-from ..runtime.device import Runtime, canonical_dtype
+from ..runtime.device import Runtime, canonical_cache_dtype, canonical_dtype
 from ..sampling.sampler import DeviceSampler, SamplingParams, fresh_seed, uniform
 from .loading import load_model, random_model
 from .model import Model
@@ -67,9 +67,12 @@ class Engine:
                  num_blocks: Optional[int] = None, max_batch_tokens: int = 4096,
                  max_batch_seqs: int = 64, prefill_chunk_size: int = 512,
                  max_seq_len: Optional[int] = None, device_index: int = 0, tuned: bool = True,
-                 use_graphs: bool = True, quiet: bool = True, decode_run: int = 4):
+                 use_graphs: bool = True, quiet: bool = True, decode_run: int = 4, cache_dtype: Optional[str] = None):
+        """``cache_dtype``: "int8" or "float8_e4m3" holds the cached keys and values in 8 bits (see StepRunner); None:
+        in the compute type."""
         self.rt = Runtime.get(device_index)
         self.dtype = canonical_dtype(dtype)
+        self.cache_dtype = canonical_cache_dtype(cache_dtype, self.dtype)
         self.model = load_model(model, self.dtype, self.rt, tuned=tuned) if isinstance(model, str) else model
         max_len = min(max_seq_len or self.model.plan.max_position, self.model.plan.max_position)
         pages = self._pages_per_group(num_blocks, block_size, max_batch_seqs, max_len,
@@ -77,7 +80,7 @@ class Engine:
         self.runner = StepRunner(self.model, self.rt, self.dtype, page_size=block_size,
                                  num_pages=pages, max_seqs=max_batch_seqs,
                                  max_batch_tokens=max_batch_tokens, max_model_len=max_len,
-                                 use_graphs=use_graphs)
+                                 use_graphs=use_graphs, cache_dtype=self.cache_dtype)
         self.scheduler = Scheduler(SchedulerConfig(max_batch_tokens, prefill_chunk_size, max_batch_seqs),
                                    self.runner.manager)
         self.sampler = DeviceSampler(self.rt, self.runner.k, max_batch_seqs)
@@ -107,6 +110,11 @@ class Engine:
         groups = group_needs(needs)
         item = 2 if self.dtype == "bfloat16" else 4
         def bytes_per_page(g):
+            if self.cache_dtype is not None:
+                # codes of whole blocks of 64 channels and two scales a token and head; and per group, for each size of heads, one layer's
+                # page in the compute type to read back into
+                heads = [(needs[c].num_kv_heads, needs[c].head_dim) for c in g.calls]
+                return block_size * (sum(n * (2 * -(-hd // 64) * 64 + 8) for n, hd in heads) + sum(n * 2 * hd * item for n, hd in set(heads)))
             return sum(needs[c].num_kv_heads * (needs[c].head_dim + (0 if getattr(needs[c], "values_in_keys", False)
                                                               else (needs[c].value_dim or needs[c].head_dim)))
                        for c in g.calls) * item * block_size

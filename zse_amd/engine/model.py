@@ -22,7 +22,20 @@ class CallCache:
     state_bytes: int = 0
     shared: bool = False             # k, v and group are another entry's (this entry stores none)
     lent: bool = False               # other entries read this entry's k and v
+    # a cache in 8 bits (see cache_q8.hip): k and v are codes, with a scale per token, head and side; the pages that a step's
+    # portions see are read back into work_k and work_v, which the layers of a group share
+    format: Optional[int] = None
+    scales: Optional[Tensor] = None  # [pages, kv heads, 2, page size] float
+    work_k: Optional[Tensor] = None
+    work_v: Optional[Tensor] = None
     extra: Dict[str, tuple] = field(default_factory=dict)   # states of the layer's other parts: key -> (offset, bytes)
+
+
+    def nbytes(self) -> int:
+        """Of the keys and values that the entry owns."""
+        if self.k is None or self.shared:
+            return 0
+        return self.k.nbytes + (0 if self.v is self.k else self.v.nbytes) + (self.scales.nbytes if self.scales is not None else 0)
 
 
 class Model:

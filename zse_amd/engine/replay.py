@@ -51,6 +51,8 @@ def main(argv: Optional[list] = None) -> int:
     ap.add_argument("--max-seqs", type=int, default=4, help="state slots: the most requests live at a time")
     ap.add_argument("--plain", action="store_true",
                     help="bfloat16 only: the plain kernels instead of the tuned ones")
+    ap.add_argument("--cache-dtype", default=None, choices=["int8", "float8_e4m3"],
+                    help="hold cached keys and values in 8 bits (default: in the compute type)")
     a = ap.parse_args(argv)
 
     from ..runtime.device import Runtime
@@ -63,7 +65,7 @@ def main(argv: Optional[list] = None) -> int:
     max_len = min(model.plan.max_position, max(a.max_tokens, 64))
     runner = StepRunner(model, rt, a.dtype, page_size=a.block_size, cache_tokens=a.max_tokens,
                         max_seqs=a.max_seqs, max_batch_tokens=max(a.max_tokens, 64),
-                        max_model_len=max_len, use_graphs=False)
+                        max_model_len=max_len, use_graphs=False, cache_dtype=a.cache_dtype)
     print(f"[trace_run] ready: {model.plan.architecture}, {len(model.plan.order)} layer calls, "
           f"pages of {a.block_size}", file=sys.stderr, flush=True)
     replay(runner, sys.stdin, a.out, log=sys.stdout)

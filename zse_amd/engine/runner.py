@@ -30,7 +30,8 @@ from ..cache.manager import CacheManager, GroupInfo, group_needs
 from ..cache.pages import OutOfPages
 from ..parts.base import PagedKV, StateNeed
 from ..parts.ops import MEMORY_SIDE_CACHE
-from ..runtime.device import BF16, F32, I32, ITEMSIZE, Runtime, Tensor, canonical_dtype
+from ..runtime.device import (BF16, CACHE_FORMATS, F32, I32, ITEMSIZE, U8, Runtime, Tensor, canonical_cache_dtype,
+                              canonical_dtype)
 from .model import CallCache, Model
 
 
@@ -112,6 +113,7 @@ class StepContext:
         self.gemm_workspace = runner.gemm_workspace
         self.weights_read_once = runner.weights_read_once
         self.cache_token_bytes = runner.cache_token_bytes
+        self.cache_dtype = runner.cache_dtype      # None: the cache holds the compute type
         self.T = 0
         self.R = 0
         self.tokens = self.positions = self.req_of_token = self.q_start = self.ctx_len = 0
@@ -137,9 +139,13 @@ class StepRunner:
                  num_pages: Optional[int] = None, cache_tokens: Optional[int] = None,
                  max_seqs: int = 64, max_batch_tokens: int = 4096, max_model_len: Optional[int] = None,
                  tuned: Optional[bool] = None, use_graphs: bool = True, use_steplists: bool = True,
-                 graph_max_batch: int = 16):
+                 graph_max_batch: int = 16, cache_dtype: Optional[str] = None):
+        """``cache_dtype``: "int8" or "float8_e4m3" holds keys and values in 8 bits with a float scale per
+        token and head (None: in the compute type); single tokens attend to the codes, a prompt's portions to
+        pages read back into the compute type.  Refused where a mixer of the model does not serve it."""
         self.model, self.rt = model, rt
         self.dtype = canonical_dtype(dtype)
+        self.cache_dtype = canonical_cache_dtype(cache_dtype, self.dtype)
         if model.loaded_dtype != self.dtype:
             raise ValueError(f"the model's weights are {model.loaded_dtype}, the runner wants {self.dtype}")
         self.k = rt.kernels(self.dtype)
@@ -181,7 +187,9 @@ class StepRunner:
         for gid, g in enumerate(groups):
             for c in g.calls:
                 gid_of[c] = gid
-        item = ITEMSIZE[self.dtype]
+        if self.cache_dtype is not None:
+            self._check_cache_dtype(needs)
+        work = {}                # the slabs that pages of a cache in 8 bits are read back into, shared by the layers of a group
         for i, need in enumerate(needs):
             cc = CallCache(need=need)
             call = model.plan.order[i]
@@ -191,8 +199,9 @@ class StepRunner:
                 # never written, it is what kernels read where a table names no page
                 pages = groups[cc.group].num_pages + 1
                 shape = (pages, need.num_kv_heads, self.page_size, need.head_dim)
-                cc.k = rt.zeros(shape, self.dtype)
                 mixer = model.blocks[call.layer].mixer
+                if self.cache_dtype is None:
+                    cc.k = rt.zeros(shape, self.dtype)
                 cc.v_transposed = bool(self.tuned and getattr(mixer, "wants_v_transposed", None) and
                                        mixer.wants_v_transposed(self.k, self.dtype, self.page_size))
                 vd = need.value_dim or need.head_dim
@@ -200,8 +209,11 @@ class StepRunner:
                 shape = (pages, nv, self.page_size, vd)
                 if cc.v_transposed:
                     shape = (pages, nv, vd, self.page_size)
-                # values that are part of the keys have no slab of their own
-                cc.v = cc.k if getattr(need, "values_in_keys", False) else rt.zeros(shape, self.dtype)
+                if self.cache_dtype is not None:
+                    self._make_q8(cc, pages, need, shape, work)
+                else:
+                    # values that are part of the keys have no slab of their own
+                    cc.v = cc.k if getattr(need, "values_in_keys", False) else rt.zeros(shape, self.dtype)
                 if getattr(need, "state_bytes", 0):      # a mixer that keeps a state beside its pages
                     cc.state_offset = slot_bytes
                     cc.state_bytes = int(need.state_bytes)
@@ -215,6 +227,7 @@ class StepRunner:
                 # beside whatever state of its own it keeps
                 own = self.caches[call.cache_of]
                 cc.need, cc.group, cc.k, cc.v, cc.v_transposed = own.need, own.group, own.k, own.v, own.v_transposed
+                cc.format, cc.scales, cc.work_k, cc.work_v = own.format, own.scales, own.work_k, own.work_v
                 cc.shared = own.lent = True
             # what the layer's other parts keep per request (a convolution's last rows, say)
             block = model.blocks[call.layer]
@@ -235,7 +248,8 @@ class StepRunner:
         # clears a page in all of them
         self._slabs = []
         for gid in range(len(groups)):
-            ts = [t for cc in self.caches if cc.group == gid and cc.k is not None and not cc.shared
+            # (the kernels of a cache in 8 bits never use what lies behind a request's last token)
+            ts = [t for cc in self.caches if cc.group == gid and cc.k is not None and not cc.shared and cc.format is None
                   for t in ((cc.k,) if cc.v is cc.k else (cc.k, cc.v))]
             ptrs = rt.upload(np.array([t.ptr for t in ts], dtype=np.uint64).view(np.float64), "float64")
             sizes = rt.upload(np.array([t.nbytes // t.shape[0] for t in ts], dtype=np.uint64).view(np.float64), "float64")
@@ -257,6 +271,10 @@ class StepRunner:
                 need = max(need, int(part.prepare(*limits, max_batch_tokens=self.max_batch_tokens)))
             else:
                 need = max(need, int(part.prepare(*limits)))
+        if self.cache_dtype is not None:
+            for call, cc in zip(model.plan.order, self.caches):
+                if cc.format is not None:
+                    need = max(need, int(model.blocks[call.layer].mixer.q8_workspace(*limits)))
         try:
             self.workspace = rt.zeros((max(need // 4 + 1, 64),), F32)
         except Exception as e:
@@ -266,8 +284,7 @@ class StepRunner:
         # a model larger than the cache on the memory's side leaves nothing of a step's weights there for the next step
         self.weights_read_once = getattr(model, "weight_bytes", 0) > MEMORY_SIDE_CACHE
         # what a token of one request has in all layers' pages
-        self.cache_token_bytes = sum((c.k.nbytes + (0 if c.v is c.k else c.v.nbytes)) // (c.k.shape[0] * self.page_size)
-                                     for c in self.caches if c.k is not None and not c.shared)
+        self.cache_token_bytes = sum(c.nbytes() // (c.k.shape[0] * self.page_size) for c in self.caches if c.k is not None)
         self.gemm_workspace = None
         if self.dtype == BF16 and self.k.has("zk_gemm_bf16_workspace"):
             self.gemm_workspace = rt.zeros((self.k.zk_gemm_bf16_workspace() // 4,), F32)
@@ -307,7 +324,32 @@ class StepRunner:
         return 4 * T + (R + 1) + 4 * R + G * (T + R * self.max_blocks) + 64
 
     def cache_bytes(self) -> int:
-        return sum(c.k.nbytes + (0 if c.v is c.k else c.v.nbytes) for c in self.caches if c.k is not None and not c.shared)
+        work = {t.ptr: t.nbytes for c in self.caches for t in (c.work_k, c.work_v) if t is not None}
+        return sum(c.nbytes() for c in self.caches) + sum(work.values())
+
+    def _check_cache_dtype(self, needs) -> None:
+        """Every mixer that keeps or reads pages has to serve a cache in 8 bits."""
+        if self.page_size % 16:
+            raise ValueError(f"a cache of {self.cache_dtype} has pages of 16, 32, 48, ... tokens, got {self.page_size}")
+        for i, (call, need) in enumerate(zip(self.model.plan.order, needs)):
+            if not isinstance(need, PagedKV) and call.cache_of is None:
+                continue
+            mixer = self.model.blocks[call.layer].mixer
+            if not (hasattr(mixer, "serves_q8") and mixer.serves_q8()):
+                raise ValueError(f"cache_dtype {self.cache_dtype}: the mixer of layer {call.layer} ({type(mixer).__name__}) does not "
+                                 f"serve a cache in 8 bits")
+
+    def _make_q8(self, cc: CallCache, pages: int, need: PagedKV, v_shape, work) -> None:
+        """The slabs of one entry's cache in 8 bits; ``work``: those to read back into that were made before."""
+        nkv, hd = need.num_kv_heads, need.head_dim
+        room = self.k.zk_cache_q8_bytes(pages, nkv, hd, self.page_size) // (pages * nkv * self.page_size)     # channels, filled up
+        cc.format = CACHE_FORMATS[self.cache_dtype]
+        cc.k, cc.v = (self.rt.zeros((pages, nkv, self.page_size, room), U8) for _ in range(2))
+        cc.scales = self.rt.zeros((pages, nkv, 2, self.page_size), F32)
+        key = (cc.group, nkv, hd, v_shape)
+        if key not in work:
+            work[key] = (self.rt.zeros((pages, nkv, self.page_size, hd), self.dtype), self.rt.zeros(v_shape, self.dtype))
+        cc.work_k, cc.work_v = work[key]
 
     # ------------------------------------------------------------------ requests
     def _clear_slot(self, req, slot: int) -> None:

@@ -232,6 +232,68 @@ class PagedAttention(Part):
             need = (need + 255) // 256 * 256 + min(extra, self.PORTION_RANGES_BYTES)
         return need
 
+    # ---- a cache in 8 bits
+    # The attention of portions reads whole tiles of keys, from a multiple of the tile on, and masks what a row does not see: pages
+    # are read back from so many positions in front of the window on, so that such a tile meets this request's own keys.
+    Q8_READ_BEFORE = 256
+
+    def serves_q8(self) -> bool:
+        """Whether this mixer keeps its keys and values in 8 bits where the runner asks for it: the plain order of product, rotation,
+        store and attention does (window, soft cap, a step of its own before the rotation); anything else in between does not."""
+        return not self.general and type(self).forward is PagedAttention.forward
+
+    def q8_workspace(self, kernels, dtype, max_seqs, max_model_len, page_size) -> int:
+        blocks = -(-int(max_model_len) // page_size)
+        return int(kernels.zk_attention_q8_workspace(int(max_seqs), self.spec.num_heads, self.spec.head_dim, blocks * page_size,
+                                                     blocks * page_size))
+
+    def _forward_q8(self, ctx, x: Tensor, cache) -> Tensor:
+        """Over a cache in 8 bits: keys and values are stored as codes as they are rotated, requests that bring one token attend to the
+        codes, and what the other requests see is read back into pages of the compute type for the attention of portions."""
+        s, k = self.spec, ctx.k
+        T, (nh, nkv, hd) = x.shape[0], (s.num_heads, s.num_kv_heads, s.head_dim)
+        n_store = 0 if self.shared_kv else nkv
+        width, item = (nh + 2 * n_store) * hd, ITEMSIZE[ctx.dtype]
+        g = ctx.group(cache.group)
+        pages = cache.k.shape[0]
+        tables = self.position.rotary_tables()
+        hooked = type(self).between_product_and_rotation is not PagedAttention.between_product_and_rotation
+        qkv = ctx.alloc((T, width))
+        got = linear(ctx, x, self.w_qkv, qkv, sums_ok=not hooked and tables is not None)
+        if hooked:
+            self.between_product_and_rotation(ctx, qkv)
+        if tables is None:
+            self.position.apply(ctx, qkv, nh, n_store, hd)
+        parts = got.layout == "parts"
+        k.zk_rope_cache_write_q8(qkv.ptr, width, got.ptr if parts else None, got.shape[0] if parts else 0, qkv.ptr, width, ctx.positions,
+                                 None if self.shared_kv else g.slot_map, tables[0].ptr if tables is not None else None,
+                                 tables[1] if tables is not None else 0, cache.k.ptr, cache.v.ptr, cache.scales.ptr, T, nh, n_store, hd,
+                                 g.page_size, pages, cache.format, ctx.stream)
+        o = ctx.alloc((T, nh * hd))
+        cap = float(s.softcap) if s.softcap else 0.0
+        win = int(s.window) if s.window else 0
+        n, single = ctx.n_multi, ctx.R - ctx.n_multi        # requests of several tokens come first
+        first = T - single
+        if n:
+            k.zk_cache_read_q8(cache.k.ptr, cache.v.ptr, cache.scales.ptr, g.block_table, g.max_blocks, ctx.q_start, ctx.ctx_len,
+                               cache.work_k.ptr, cache.work_v.ptr, n, ctx.max_ctx, win + self.Q8_READ_BEFORE if win else 0, nkv, hd,
+                               g.page_size, pages, 1 if cache.v_transposed else 0, cache.format, ctx.stream)
+            if cache.v_transposed and ctx.tuned:
+                k.zk_attention_bf16_once(qkv.ptr, width, cache.work_k.ptr, cache.work_v.ptr, g.block_table, g.max_blocks, ctx.q_start,
+                                         ctx.ctx_len, o.ptr, n, n, ctx.max_q_len, ctx.max_ctx, nh, nkv, hd, g.page_size, s.scale, cap,
+                                         win, self.decode_chunk, ctx.workspace.ptr, ctx.workspace.nbytes, 0, 0, 0, 0, hd, 0, None, None,
+                                         0, getattr(ctx, "portion_ctx", 0), 0, ctx.stream)
+            else:
+                k.zk_attention_plain(qkv.ptr, width, cache.work_k.ptr, cache.work_v.ptr, g.block_table, g.max_blocks, ctx.req_of_token,
+                                     ctx.positions, o.ptr, first, nh, nkv, hd, g.page_size, s.scale, cap, win,
+                                     1 if cache.v_transposed else 0, ctx.stream)
+        if single:
+            k.zk_attention_q8(qkv.ptr + first * width * item, width, cache.k.ptr, cache.v.ptr, cache.scales.ptr,
+                              g.block_table + n * g.max_blocks * 4, g.max_blocks, ctx.ctx_len + n * 4, o.ptr + first * nh * hd * item,
+                              single, ctx.max_ctx, nh, nkv, hd, g.page_size, pages, s.scale, cap, win, cache.format, ctx.workspace.ptr,
+                              ctx.workspace.nbytes, ctx.stream)
+        return linear(ctx, o, self.w_o, ctx.alloc((T, s.hidden_size)), last_of=self)
+
     def between_product_and_rotation(self, ctx, qkv: Tensor) -> None:
         """A mixer that differs from this one only in what it does to queries and keys before
         they are rotated and stored (a norm over each head, say) overrides this and changes
@@ -336,6 +398,7 @@ class PagedAttention(Part):
         s, tables = self.spec, self.position.rotary_tables()
         width = (s.num_heads + 2 * (0 if self.shared_kv else s.num_kv_heads)) * s.head_dim
         return bool(not self.general and type(self).forward is PagedAttention.forward and size == s.hidden_size and
+                    getattr(ctx, "cache_dtype", None) is None and
                     type(self).between_product_and_rotation is PagedAttention.between_product_and_rotation and
                     tables is not None and tuned_gemm(ctx, s.hidden_size) and self.w_qkv.layout == "strip" and
                     ctx.k.zk_qkv_rope_bf16_supports(1, s.hidden_size, s.head_dim, tables[1]) and
@@ -344,6 +407,8 @@ class PagedAttention(Part):
     def forward(self, ctx, x: Tensor, cache) -> Tensor:
         if self.general:
             return self._forward_general(ctx, x, cache)
+        if getattr(cache, "format", None) is not None:
+            return self._forward_q8(ctx, x, cache)
         s, k = self.spec, ctx.k
         T = x.shape[0]
         nh, nkv, hd = s.num_heads, s.num_kv_heads, s.head_dim

@@ -26,6 +26,24 @@ NUMPY_OF = {F32: np.float32, BF16: np.uint16, I32: np.int32, F64: np.float64, U8
 DTYPE_ALIASES = {"float32": F32, "fp32": F32, "f32": F32, "bfloat16": BF16, "bf16": BF16}
 
 
+# what a cache in 8 bits holds -> the kernels' number of it
+CACHE_FORMATS = {"int8": 0, "float8_e4m3": 1}
+CACHE_ALIASES = {"fp8": "float8_e4m3", "e4m3": "float8_e4m3"}
+
+
+def canonical_cache_dtype(name: Optional[str], dtype: str) -> Optional[str]:
+    """None where the cache holds the compute type ``dtype``, else the name of its 8-bit format."""
+    if name is None:
+        return None
+    low = str(name).lower()
+    if DTYPE_ALIASES.get(low) == canonical_dtype(dtype):
+        return None
+    low = CACHE_ALIASES.get(low, low)
+    if low not in CACHE_FORMATS:
+        raise ValueError(f"cache_dtype must be one of {sorted(CACHE_FORMATS)} or the compute type, got {name!r}")
+    return low
+
+
 def canonical_dtype(name: str) -> str:
     try:
         return DTYPE_ALIASES[str(name).lower()]
