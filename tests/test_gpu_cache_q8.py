@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 HALF = {"bfloat16": 2.0 ** -8, "float32": 2.0 ** -24}
 # query heads, key heads, channels, tokens of a page
 SHAPES = [(8, 4, 256, 16), (4, 2, 128, 32), (12, 12, 64, 16), (20, 4, 96, 48), (32, 1, 128, 64), (5, 5, 80, 16), (34, 2, 40, 16), (3, 1, 7, 16),
-          (18, 1, 192, 128), (6, 3, 200, 16)]
+          (18, 1, 192, 128), (6, 3, 200, 16), (32, 2, 256, 16)]
 
 
 @pytest.fixture(scope="module")

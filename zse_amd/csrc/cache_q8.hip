@@ -100,6 +100,7 @@ __device__ __forceinline__ void q8_sincos(float pos, float freq, float& sn, floa
 
 typedef float q8_f4 __attribute__((ext_vector_type(4)));
 typedef unsigned q8_u4 __attribute__((ext_vector_type(4)));
+typedef act_t q8_a4 __attribute__((ext_vector_type(4)));
 #if ZSE_ACT_BF16
 typedef __bf16 q8_b8 __attribute__((ext_vector_type(8)));
 typedef __bf16 q8_b2 __attribute__((ext_vector_type(2)));
@@ -133,23 +134,18 @@ struct Q8Rows {
   const float* planes;        // partial sums of a split product
   int ld, sums;
   size_t plane;
-  __device__ __forceinline__ float at(size_t i) const {
-    if constexpr (!SUMS) return to_f32(rows[i]);
+  __device__ __forceinline__ act_t at(size_t i) const {
+    if constexpr (!SUMS) return rows[i];
     float x = planes[i];
     for (int p = 1; p < sums; p++) x += planes[p * plane + i];
-    return to_f32(from_f32<act_t>(x));
+    return from_f32<act_t>(x);
   }
-  __device__ __forceinline__ void at4(size_t i, float (&v)[4]) const {
-    typedef act_t a4 __attribute__((ext_vector_type(4)));
-    if constexpr (!SUMS) {
-      const a4 x = *(const a4*)(rows + i);
-#pragma unroll
-      for (int e = 0; e < 4; e++) v[e] = to_f32(x[e]);
-    } else {
+  __device__ __forceinline__ q8_a4 at4(size_t i) const {
+    if constexpr (!SUMS) return *(const q8_a4*)(rows + i);
+    else {
       q8_f4 x = *(const q8_f4*)(planes + i);
       for (int p = 1; p < sums; p++) x += *(const q8_f4*)(planes + p * plane + i);
-#pragma unroll
-      for (int e = 0; e < 4; e++) v[e] = to_f32(from_f32<act_t>(x[e]));
+      return q8_a4{from_f32<act_t>(x[0]), from_f32<act_t>(x[1]), from_f32<act_t>(x[2]), from_f32<act_t>(x[3])};
     }
   }
 };
@@ -201,10 +197,16 @@ __global__ __launch_bounds__(256, WHOLE ? 4 : 2) void write_q8_kernel(Q8Write<SU
   // lane i: the slot of row t0 - 3 + i, for ten rows; bit i of ``fours``: rows i to i + 3 are such a four
   const int near = t0 - 3 + lane;
   int slots = p.slot_map && lane < 10 && near >= 0 && near < p.T ? p.slot_map[near] : -1;
+  const float position = lane < 10 && near >= 0 && near < p.T ? (float)p.positions[near] : 0.f;
   if (slots >= 0 && slots / p.bs >= p.num_pages) slots = -1;
   const int s1 = __shfl(slots, lane + 1), s2 = __shfl(slots, lane + 2), s3 = __shfl(slots, lane + 3);
   const unsigned fours = (unsigned)__ballot(lane < 7 && slots >= 0 && slots % 4 == 0 && s1 == slots + 1 && s2 == slots + 2 && s3 == slots + 3);
   const int page = slots >= 0 ? slots / p.bs : 0, off = slots >= 0 ? slots % p.bs : 0;
+  const size_t piece_of = ((size_t)page * p.nkv * pieces + off / Q8_PIECE) * (size_t)(blocks * Q8_BYTES);
+  const size_t scale_of = (size_t)page * p.nkv * 2 * p.bs + off;
+  auto of_row = [](size_t v, int i) {
+    return (size_t)(unsigned)__builtin_amdgcn_readlane((int)v, i) | (size_t)__builtin_amdgcn_readlane((int)(v >> 32), i) << 32;
+  };
   for (int taken = 0; taken < 2; taken++) {
     // the four that begins among the block's rows, then the block's rows that are in none
     const bool four = taken == 0;
@@ -215,50 +217,65 @@ __global__ __launch_bounds__(256, WHOLE ? 4 : 2) void write_q8_kernel(Q8Write<SU
     if (!mine) continue;
     const int start = four ? __builtin_ctz(fours & 0x78) : 3, present = start + __builtin_ctz(mine);
     int row[4], slot[4], at[4];                          // what is not there is read as a row that is, and not stored
-    size_t piece[4], scale_at[4];
+    size_t piece[4];
 #pragma unroll
     for (int t = 0; t < 4; t++) {
       const int i = mine >> t & 1 ? start + t : present;
       row[t] = t0 - 3 + i;
       slot[t] = mine >> t & 1 ? __builtin_amdgcn_readlane(slots, i) : -1;
-      const int pg = __builtin_amdgcn_readlane(page, i), o = __builtin_amdgcn_readlane(off, i);
-      at[t] = o % Q8_PIECE;
-      piece[t] = ((size_t)pg * p.nkv * pieces + o / Q8_PIECE) * (size_t)(blocks * Q8_BYTES);
-      scale_at[t] = (size_t)pg * p.nkv * 2 * p.bs + o;
+      at[t] = __builtin_amdgcn_readlane(off, i) % Q8_PIECE;
+      piece[t] = of_row(piece_of, i);
     }
+    // lane t of every quad: row t's, for its scales
+    const int quad = mine >> (lane & 3) & 1 ? start + (lane & 3) : present;
+    const int quad_slot = mine >> (lane & 3) & 1 ? __shfl(slots, quad) : -1;
+    const size_t quad_scale = (size_t)(unsigned)__shfl((int)scale_of, quad) | (size_t)__shfl((int)(scale_of >> 32), quad) << 32;
     const bool stores = slot[0] >= 0 || slot[1] >= 0 || slot[2] >= 0 || slot[3] >= 0;
     bool turned = false;
-    for (int base = blockIdx.y * HEADS; base < p.heads; base += gridDim.y * HEADS) {
-      const int head = min(base + sub, p.heads - 1);
-      const bool live = base + sub < p.heads, is_q = head < p.nh, is_v = head >= p.nh + p.nkv;
-      float x[4][4], y[4][4];                         // a row's four channels, and those that they turn with
+    const int pass = gridDim.y * HEADS;
+    q8_a4 xr[4], yr[4];                              // a row's four channels, and those that they turn with: a pass ahead
+    auto ask = [&](int base) {
+      const size_t head_at = (size_t)min(base + sub, p.heads - 1) * p.hd;
 #pragma unroll
       for (int t = 0; t < 4; t++) {
-        const size_t from = (size_t)row[t] * p.from.ld + (size_t)head * p.hd;
+        const size_t from = (size_t)row[t] * p.from.ld + head_at;
         if constexpr (WHOLE) {
-          p.from.at4(from + own, x[t]);
-          p.from.at4(from + other, y[t]);
+          xr[t] = p.from.at4(from + own);
+          yr[t] = p.from.at4(from + other);
         } else {
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             const int c = c0 + e, mate = c >= p.rotary_dim ? c : c < half ? c + half : c - half;
-            x[t][e] = p.from.at(from + (c < p.hd ? c : 0));
-            y[t][e] = p.from.at(from + (c < p.hd ? mate : 0));
+            xr[t][e] = p.from.at(from + (c < p.hd ? c : 0));
+            yr[t][e] = p.from.at(from + (c < p.hd ? mate : 0));
           }
         }
       }
+    };
+    if (blockIdx.y * HEADS < p.heads) ask(blockIdx.y * HEADS);
+    for (int base = blockIdx.y * HEADS; base < p.heads; base += pass) {
+      const int head = min(base + sub, p.heads - 1);
+      const bool live = base + sub < p.heads, is_q = head < p.nh, is_v = head >= p.nh + p.nkv;
       if (!turned && half > 0 && base < p.nh + p.nkv) {        // the first pass with queries or keys
         if (taken) __syncthreads();                            // (the other rows' angles have been read)
-        for (int t = 0; t < 4; t++)
-          if (mine >> t & 1) {
-            const float pos = (float)p.positions[t == 0 ? row[0] : t == 1 ? row[1] : t == 2 ? row[2] : row[3]];
-            // a row a wave, so that all four are worked out side by side
-            if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) == t)
-              for (int i = lane; i < half; i += 64) q8_sincos(pos, p.inv_freq[i], ((float*)s_sin[t])[i], ((float*)s_cos[t])[i]);
-          }
+        // a row a wave, so that all four are worked out side by side
+        const int t = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        if (mine >> t & 1) {
+          const float pos = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(position), start + t));
+          for (int i = lane; i < half; i += 64) q8_sincos(pos, p.inv_freq[i], ((float*)s_sin[t])[i], ((float*)s_cos[t])[i]);
+        }
         __syncthreads();
         turned = true;
       }
+      float x[4][4], y[4][4];
+#pragma unroll
+      for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          x[t][e] = to_f32(xr[t][e]);
+          y[t][e] = to_f32(yr[t][e]);
+        }
+      if (base + pass < p.heads) ask(base + pass);
       if (!is_v) {
 #pragma unroll
         for (int t = 0; t < 4; t++) {
@@ -287,8 +304,7 @@ __global__ __launch_bounds__(256, WHOLE ? 4 : 2) void write_q8_kernel(Q8Write<SU
           if (!(mine >> t & 1)) continue;
           act_t* to = p.q_out + (size_t)row[t] * p.ldq + (size_t)head * p.hd + c0;
           if constexpr (WHOLE) {
-            typedef act_t a4 __attribute__((ext_vector_type(4)));
-            if (c0 < p.hd) *(a4*)to = a4{from_f32<act_t>(x[t][0]), from_f32<act_t>(x[t][1]), from_f32<act_t>(x[t][2]), from_f32<act_t>(x[t][3])};
+            if (c0 < p.hd) *(q8_a4*)to = q8_a4{from_f32<act_t>(x[t][0]), from_f32<act_t>(x[t][1]), from_f32<act_t>(x[t][2]), from_f32<act_t>(x[t][3])};
           } else {
 #pragma unroll
             for (int e = 0; e < 4; e++)
@@ -346,11 +362,8 @@ __global__ __launch_bounds__(256, WHOLE ? 4 : 2) void write_q8_kernel(Q8Write<SU
           }
         }
       }
-      if (c0 < 16) {                                   // the head's first four lanes: a row's scale each
-        const int t = lane & 3;
-        const size_t to = t == 0 ? scale_at[0] : t == 1 ? scale_at[1] : t == 2 ? scale_at[2] : scale_at[3];
-        if ((t == 0 ? slot[0] : t == 1 ? slot[1] : t == 2 ? slot[2] : slot[3]) >= 0) p.scales[to + (size_t)(2 * kvh + is_v) * p.bs] = scale;
-      }
+      // the head's first four lanes: a row's scale each
+      if (c0 < 16 && quad_slot >= 0) p.scales[quad_scale + (size_t)(2 * kvh + is_v) * p.bs] = scale;
     }
   }
 #endif
@@ -371,7 +384,7 @@ template <int FMT, bool TRANSPOSED, bool WHOLE>
 __global__ __launch_bounds__(256) void read_q8_kernel(Q8Read p) {
 #ifdef __HIP_DEVICE_COMPILE__
   typedef unsigned u2 __attribute__((ext_vector_type(2)));
-  typedef act_t a4 __attribute__((ext_vector_type(4)));
+  typedef q8_a4 a4;
   typedef act_t a8 __attribute__((ext_vector_type(8)));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pieces = p.bs / Q8_PIECE, per_page = pieces * p.nkv;
   // the requests' pages are numbered through, 64 requests at a time: lane i knows where those of request r0 + i end
@@ -823,7 +836,9 @@ static int q8_refuses(const char* who, const void* kcodes, const void* vcodes, c
 // 128 channels by 1,024, 2,048 and 4,096 blocks 43, 40 and 38 us; more work out the same angles).  Read back: waves that take
 // pieces in turn (64 pages of 8 heads in a range of 64,512 pieces by 2,048, 4,096 and 8,192 blocks 6.2, 8.1 and 10.4 us, empty ones
 // cost as much as others; 147,000 pieces that are all there 56.9, 56.3 and 56.2).
+#ifndef Q8_WRITE_BLOCKS
 #define Q8_WRITE_BLOCKS 4096
+#endif
 #define Q8_READ_BLOCKS 2048
 
 // Calls ``go`` with what is only known at run time as a constant.
