@@ -24,7 +24,7 @@ ATTEND = dict(q=A, q_stride=1024, kcodes=A, vcodes=A, scales=A, block_table=A, m
               bs=16, num_pages=9, scale=0.1, softcap=0.0, window=0, format=0, workspace=A, workspace_bytes=1 << 30, stream=None)
 
 CACHE = [(dict(bs=8), "pages of 16"), (dict(bs=0), "pages of 16"), (dict(bs=24), "pages of 16"), (dict(num_pages=0), "one page"),
-         (dict(hd=257), "256 channels"), (dict(hd=0), ""), (dict(format=2), "format"), (dict(format=-1), "format"), (dict(kcodes=A + 8), "16"),
+         (dict(hd=257), "256 channels"), (dict(bs=1 << 23), "2 GiB"), (dict(hd=0), ""), (dict(format=2), "format"), (dict(format=-1), "format"), (dict(kcodes=A + 8), "16"),
          (dict(vcodes=None), "16"), (dict(scales=A + 4), "16")]
 
 

@@ -134,17 +134,19 @@ struct Q8Rows {
   const float* planes;        // partial sums of a split product
   int ld, sums;
   size_t plane;
-  __device__ __forceinline__ act_t at(size_t i) const {
-    if constexpr (!SUMS) return rows[i];
-    float x = planes[i];
-    for (int p = 1; p < sums; p++) x += planes[p * plane + i];
+  __device__ __forceinline__ act_t at(int row, unsigned i) const {
+    if constexpr (!SUMS) return (rows + (size_t)row * ld)[i];
+    const float* r = planes + (size_t)row * ld;
+    float x = r[i];
+    for (int p = 1; p < sums; p++) x += (r + p * plane)[i];
     return from_f32<act_t>(x);
   }
-  __device__ __forceinline__ q8_a4 at4(size_t i) const {
-    if constexpr (!SUMS) return *(const q8_a4*)(rows + i);
+  __device__ __forceinline__ q8_a4 at4(int row, unsigned i) const {
+    if constexpr (!SUMS) return *(const q8_a4*)(rows + (size_t)row * ld + i);
     else {
-      q8_f4 x = *(const q8_f4*)(planes + i);
-      for (int p = 1; p < sums; p++) x += *(const q8_f4*)(planes + p * plane + i);
+      const float* r = planes + (size_t)row * ld;
+      q8_f4 x = *(const q8_f4*)(r + i);
+      for (int p = 1; p < sums; p++) x += *(const q8_f4*)(r + p * plane + i);
       return q8_a4{from_f32<act_t>(x[0]), from_f32<act_t>(x[1]), from_f32<act_t>(x[2]), from_f32<act_t>(x[3])};
     }
   }
@@ -193,7 +195,8 @@ __global__ __launch_bounds__(256, WHOLE ? 4 : 2) void write_q8_kernel(Q8Write<SU
   const int own = c0 < p.hd ? c0 : 0, other = !rotated ? own : low ? c0 + half : c0 - half;
   const int turn_at = rotated ? (low ? c0 : c0 - half) / 4 : 0;
   const int key_at = c0 / Q8_BLOCK * Q8_BYTES + c0 % Q8_BLOCK, value_at = c0 / Q8_BLOCK * Q8_BYTES + q8_value_at(0, c0 % Q8_BLOCK);
-  const size_t head_bytes = (size_t)pieces * blocks * Q8_BYTES;
+  const unsigned sign = low ? 0x80000000u : 0u;             // a - b turns where the lane holds the pair's first
+  const unsigned head_bytes = pieces * blocks * Q8_BYTES;
   // lane i: the slot of row t0 - 3 + i, for ten rows; bit i of ``fours``: rows i to i + 3 are such a four
   const int near = t0 - 3 + lane;
   int slots = p.slot_map && lane < 10 && near >= 0 && near < p.T ? p.slot_map[near] : -1;
@@ -235,19 +238,18 @@ __global__ __launch_bounds__(256, WHOLE ? 4 : 2) void write_q8_kernel(Q8Write<SU
     const int pass = gridDim.y * HEADS;
     q8_a4 xr[4], yr[4];                              // a row's four channels, and those that they turn with: a pass ahead
     auto ask = [&](int base) {
-      const size_t head_at = (size_t)min(base + sub, p.heads - 1) * p.hd;
+      const unsigned head_at = min(base + sub, p.heads - 1) * p.hd;
 #pragma unroll
       for (int t = 0; t < 4; t++) {
-        const size_t from = (size_t)row[t] * p.from.ld + head_at;
         if constexpr (WHOLE) {
-          xr[t] = p.from.at4(from + own);
-          yr[t] = p.from.at4(from + other);
+          xr[t] = p.from.at4(row[t], head_at + own);
+          yr[t] = p.from.at4(row[t], head_at + other);
         } else {
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             const int c = c0 + e, mate = c >= p.rotary_dim ? c : c < half ? c + half : c - half;
-            xr[t][e] = p.from.at(from + (c < p.hd ? c : 0));
-            yr[t][e] = p.from.at(from + (c < p.hd ? mate : 0));
+            xr[t][e] = p.from.at(row[t], head_at + (c < p.hd ? c : 0));
+            yr[t][e] = p.from.at(row[t], head_at + (c < p.hd ? mate : 0));
           }
         }
       }
@@ -274,6 +276,7 @@ __global__ __launch_bounds__(256, WHOLE ? 4 : 2) void write_q8_kernel(Q8Write<SU
         for (int e = 0; e < 4; e++) {
           x[t][e] = to_f32(xr[t][e]);
           y[t][e] = to_f32(yr[t][e]);
+          if (WHOLE) y[t][e] = __uint_as_float(__float_as_uint(y[t][e]) ^ sign);
         }
       if (base + pass < p.heads) ask(base + pass);
       if (!is_v) {
@@ -283,7 +286,7 @@ __global__ __launch_bounds__(256, WHOLE ? 4 : 2) void write_q8_kernel(Q8Write<SU
             if (rotated) {
               const q8_f4 sn = s_sin[t][turn_at], cs = s_cos[t][turn_at];
 #pragma unroll
-              for (int e = 0; e < 4; e++) x[t][e] = __fmaf_rn(x[t][e], cs[e], __fmul_rn(y[t][e], low ? -sn[e] : sn[e]));     // as rotate_pair
+              for (int e = 0; e < 4; e++) x[t][e] = __fmaf_rn(x[t][e], cs[e], __fmul_rn(y[t][e], sn[e]));        // as rotate_pair
             }
           } else {
 #pragma unroll
@@ -302,7 +305,7 @@ __global__ __launch_bounds__(256, WHOLE ? 4 : 2) void write_q8_kernel(Q8Write<SU
 #pragma unroll
         for (int t = 0; t < 4; t++) {
           if (!(mine >> t & 1)) continue;
-          act_t* to = p.q_out + (size_t)row[t] * p.ldq + (size_t)head * p.hd + c0;
+          act_t* to = p.q_out + (size_t)row[t] * p.ldq + (unsigned)(head * p.hd + c0);
           if constexpr (WHOLE) {
             if (c0 < p.hd) *(q8_a4*)to = q8_a4{from_f32<act_t>(x[t][0]), from_f32<act_t>(x[t][1]), from_f32<act_t>(x[t][2]), from_f32<act_t>(x[t][3])};
           } else {
@@ -316,13 +319,15 @@ __global__ __launch_bounds__(256, WHOLE ? 4 : 2) void write_q8_kernel(Q8Write<SU
       float most[4];
 #pragma unroll
       for (int t = 0; t < 4; t++) {
-        unsigned a = 0;
+        if constexpr (WHOLE) {
+          if (c0 >= p.hd) x[t][0] = x[t][1] = x[t][2] = x[t][3] = 0.f;          // the last block is filled up with zeros
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          if (c0 + e >= p.hd) x[t][e] = 0.f;                   // the last block is filled up with zeros
-          a = max(a, __float_as_uint(x[t][e]) & 0x7fffffffu);
+          for (int e = 0; e < 4; e++)
+            if (c0 + e >= p.hd) x[t][e] = 0.f;
         }
-        most[t] = q8_largest<LANES>(__uint_as_float(a));
+        const float a = __builtin_elementwise_maximum(__builtin_elementwise_maximum(fabsf(x[t][0]), fabsf(x[t][1])), fabsf(x[t][2]));
+        most[t] = q8_largest<LANES>(__builtin_elementwise_maximum(a, fabsf(x[t][3])));
       }
       // a lane works out one row's factor for the four lanes of its quad
       float scale, factor;
@@ -339,27 +344,28 @@ __global__ __launch_bounds__(256, WHOLE ? 4 : 2) void write_q8_kernel(Q8Write<SU
       }
       if (is_q || !live) continue;
       const int kvh = (head - p.nh) - (is_v ? p.nkv : 0);
-      uint8_t* codes = (is_v ? p.vcodes : p.kcodes) + kvh * head_bytes;
-      if (!padded) {
-        if (is_v && four) {
-          // the four rows' bytes of a channel side by side
-          const unsigned a = __builtin_amdgcn_perm(word[1], word[0], 0x05010400), b = __builtin_amdgcn_perm(word[1], word[0], 0x07030602);
-          const unsigned d = __builtin_amdgcn_perm(word[3], word[2], 0x05010400), f = __builtin_amdgcn_perm(word[3], word[2], 0x07030602);
-          unsigned* to = (unsigned*)(codes + piece[0] + value_at + at[0] * 64);      // (the next channel: 16 bytes on)
-          to[0] = __builtin_amdgcn_perm(d, a, 0x05040100);
-          to[4] = __builtin_amdgcn_perm(d, a, 0x07060302);
-          to[8] = __builtin_amdgcn_perm(f, b, 0x05040100);
-          to[12] = __builtin_amdgcn_perm(f, b, 0x07060302);
-        } else {
+      const unsigned head_at = kvh * head_bytes;
+      if (padded) {
+      } else if (!is_v) {
 #pragma unroll
-          for (int t = 0; t < 4; t++) {
-            if (slot[t] < 0) continue;
-            if (is_v) {
-              uint8_t* to = codes + piece[t] + value_at + at[t] / 4 * 256 + at[t] % 4;
+        for (int t = 0; t < 4; t++)
+          if (slot[t] >= 0) *(unsigned*)(p.kcodes + piece[t] + at[t] * 64 + (head_at + key_at)) = word[t];
+      } else if (four) {
+        // the four rows' bytes of a channel side by side
+        const unsigned a = __builtin_amdgcn_perm(word[1], word[0], 0x05010400), b = __builtin_amdgcn_perm(word[1], word[0], 0x07030602);
+        const unsigned d = __builtin_amdgcn_perm(word[3], word[2], 0x05010400), f = __builtin_amdgcn_perm(word[3], word[2], 0x07030602);
+        uint8_t* to = p.vcodes + piece[0] + at[0] * 64 + (head_at + value_at);          // (the next channel: 16 bytes on)
+        *(unsigned*)to = __builtin_amdgcn_perm(d, a, 0x05040100);
+        *(unsigned*)(to + 16) = __builtin_amdgcn_perm(d, a, 0x07060302);
+        *(unsigned*)(to + 32) = __builtin_amdgcn_perm(f, b, 0x05040100);
+        *(unsigned*)(to + 48) = __builtin_amdgcn_perm(f, b, 0x07060302);
+      } else {
 #pragma unroll
-              for (int e = 0; e < 4; e++) to[16 * e] = (uint8_t)(word[t] >> (8 * e));
-            } else *(unsigned*)(codes + piece[t] + key_at + at[t] * 64) = word[t];
-          }
+        for (int t = 0; t < 4; t++) {
+          if (slot[t] < 0) continue;
+          uint8_t* to = p.vcodes + piece[t] + (at[t] / 4 * 256 + at[t] % 4) + (head_at + value_at);
+#pragma unroll
+          for (int e = 0; e < 4; e++) to[16 * e] = (uint8_t)(word[t] >> (8 * e));
         }
       }
       // the head's first four lanes: a row's scale each
@@ -825,6 +831,7 @@ static int q8_refuses(const char* who, const void* kcodes, const void* vcodes, c
   const char* why = nullptr;
   if (nkv <= 0 || hd <= 0 || hd > 256) why = "1 to 256 channels of one key head or more";
   else if (bs <= 0 || bs % Q8_PIECE != 0 || num_pages <= 0) why = "pages of 16, 32, 48, ... tokens, one page or more";
+  else if ((long long)nkv * bs * q8_blocks(hd) * Q8_BLOCK >= (1ll << 31)) why = "pages of less than 2 GiB";
   else if (format != 0 && format != 1) why = "format 0 (int8) or 1 (e4m3)";
   else if (!kcodes || !vcodes || !scales || ((uintptr_t)kcodes | (uintptr_t)vcodes | (uintptr_t)scales) % 16 != 0)
     why = "codes and scales at addresses that are multiples of 16";
