@@ -481,6 +481,7 @@ struct Q8Attention {
   float *part_o, *part_ml;          // [R][nh][splits][channels, filled up] and [..][2]
   int q_stride, max_blocks, max_ctx, nh, nkv, hd, pieces, num_pages, window, chunk, q_whole;
   float k1, k2, c2;                 // z log2(e) = k1 dot, or c2 tanh(k2 dot)
+  float rest;                       // what k1, or c2, is short of its value
 };
 
 #if ZSE_ACT_BF16
@@ -517,11 +518,12 @@ __global__ __launch_bounds__(256, 2) void attention_q8_kernel(Q8Attention p) {
 #ifdef __HIP_DEVICE_COMPILE__
   extern __shared__ float s_join[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-  const int group = p.nh / p.nkv, kvh = blockIdx.y % p.nkv, head0 = blockIdx.y / p.nkv * 16, r = blockIdx.z;
-  const int heads = min(16, group - head0), splits = gridDim.x;
-  // neighbouring blocks go to different XCDs: turned by request and head, so that no XCD has one chunk of every request (with eight
-  // chunks 64 requests of uneven lengths took 74 us instead of 59)
-  const int split = (blockIdx.x + blockIdx.y + r) % splits;
+  // Chunks are the slowest index, the one that the window cuts the last: what is left for a last round of blocks is chunks that
+  // requests have little of (64 requests of 200 to 3,840 keys 56.2 -> 55.1 us, eight of 8,192 48.6 -> 47.3; with chunks as the fastest
+  // index and eight of them a request, an XCD had the same chunk of all requests: 74 us).  Neighbouring blocks go to different
+  // XCDs: requests are turned by the chunk, so that none has one request alone.
+  const int splits = gridDim.z, split = p.window > 0 ? (blockIdx.z + 1) % splits : blockIdx.z, r = (blockIdx.y + blockIdx.z) % gridDim.y;
+  const int group = p.nh / p.nkv, kvh = blockIdx.x % p.nkv, head0 = blockIdx.x / p.nkv * 16, heads = min(16, group - head0);
   // without a window the chunk's place in the table does not wait for the request's length
   int early = -1;
   if (p.window == 0 && p.max_ctx > 0) early = p.block_table[(size_t)r * p.max_blocks + min((split * (p.chunk / Q8_PIECE) + lane) / p.pieces, p.max_blocks - 1)];
@@ -615,9 +617,15 @@ __global__ __launch_bounds__(256, 2) void attention_q8_kernel(Q8Attention p) {
   for (int pair = wave; pair < n_pairs; pair += 4) {
     // scores of head col: keys 16 (p0 + 2 pair + u) + 4 g + i
     float z[2][4];
+#if !ZSE_ACT_BF16
+    float val[2][4];                 // z by its factor: the exponent below is taken from these with one rounding
+#endif
 #pragma unroll
     for (int u = 0; u < 2; u++) {
       q8_f4 s = {0.f, 0.f, 0.f, 0.f};
+#if !ZSE_ACT_BF16
+      q8_f4 s2 = s;                                    // two chains of sums: shorter, and side by side
+#endif
 #pragma unroll
       for (int j = 0; j < NB; j++) {
 #if ZSE_ACT_BF16
@@ -629,10 +637,16 @@ __global__ __launch_bounds__(256, 2) void attention_q8_kernel(Q8Attention p) {
           float x[4];
           q8_floats<FMT>(kc[u][j][w], x);
 #pragma unroll
-          for (int e = 0; e < 4; e++) s = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], qf[j][4 * w + e], s, 0, 0, 0);
+          for (int e = 0; e < 4; e++) {
+            q8_f4& sum = e & 1 ? s2 : s;
+            sum = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], qf[j][4 * w + e], sum, 0, 0, 0);
+          }
         }
 #endif
       }
+#if !ZSE_ACT_BF16
+      s += s2;
+#endif
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const float dot = s[i] * ks[u][i];
@@ -640,9 +654,15 @@ __global__ __launch_bounds__(256, 2) void attention_q8_kernel(Q8Attention p) {
 #if ZSE_ACT_BF16
           z[u][i] = p.c2 - 2.f * p.c2 * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(p.k2 * dot) + 1.f);
 #else
-          z[u][i] = p.c2 * tanhf(p.k2 * dot);
+          val[u][i] = tanhf(p.k2 * dot);
+          z[u][i] = p.c2 * val[u][i];
 #endif
-        } else z[u][i] = p.k1 * dot;
+        } else {
+          z[u][i] = p.k1 * dot;
+#if !ZSE_ACT_BF16
+          val[u][i] = dot;
+#endif
+        }
       }
     }
     if (pair + 4 < n_pairs) {
@@ -691,7 +711,13 @@ __global__ __launch_bounds__(256, 2) void attention_q8_kernel(Q8Attention p) {
     for (int u = 0; u < 2; u++)
 #pragma unroll
       for (int i = 0; i < 4; i++) {
+#if ZSE_ACT_BF16
         const float e = __builtin_amdgcn_exp2f(z[u][i] - base);
+#else
+        // a rounding of z is |z| 2^-24 of its weight, as much as everything else together
+        const float by = __fmaf_rn(val[u][i], CAP ? p.c2 : p.k1, -base) + val[u][i] * p.rest;
+        const float e = z[u][i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(by);
+#endif
         l += e;
         w[u][i] = e * vs[u][i];
       }
@@ -774,7 +800,7 @@ __global__ __launch_bounds__(256, 2) void attention_q8_kernel(Q8Attention p) {
 // behind its chunks is never used).
 template <int NB>
 __global__ __launch_bounds__(256) void attention_q8_join_kernel(Q8Attention p, int splits) {
-  constexpr int LANES = NB * 16, GROUPS = 256 / LANES, AHEAD = 4;
+  constexpr int LANES = NB * 16, GROUPS = 256 / LANES, AHEAD = 8;
   __shared__ float s_o[GROUPS][NB * 64];
   const int head = blockIdx.x, r = blockIdx.y, lane = threadIdx.x & 63, group = min((int)threadIdx.x / LANES, GROUPS - 1), at = threadIdx.x % LANES;
   const size_t row = ((size_t)r * p.nh + head) * splits;
@@ -843,9 +869,7 @@ static int q8_refuses(const char* who, const void* kcodes, const void* vcodes, c
 // 128 channels by 1,024, 2,048 and 4,096 blocks 43, 40 and 38 us; more work out the same angles).  Read back: waves that take
 // pieces in turn (64 pages of 8 heads in a range of 64,512 pieces by 2,048, 4,096 and 8,192 blocks 6.2, 8.1 and 10.4 us, empty ones
 // cost as much as others; 147,000 pieces that are all there 56.9, 56.3 and 56.2).
-#ifndef Q8_WRITE_BLOCKS
 #define Q8_WRITE_BLOCKS 4096
-#endif
 #define Q8_READ_BLOCKS 2048
 
 // Calls ``go`` with what is only known at run time as a constant.
@@ -942,6 +966,7 @@ int zk_cache_read_q8(const void* kcodes, const void* vcodes, const float* scales
   ZK_REQUIRE(nkv <= 65535 && R <= 65535, "zk_cache_read_q8: too many requests or heads");
   if (R == 0 || max_ctx == 0) return 0;
   ZK_REQUIRE(block_table && ctx_len && k && v && ((uintptr_t)k | (uintptr_t)v) % 16 == 0, "zk_cache_read_q8: null or misaligned argument");
+  if (window >= max_ctx) window = 0;                   // (sums of ctx, rows and window stay in 32 bits)
   Q8Read p;
   p.kcodes = (const uint8_t*)kcodes;
   p.vcodes = (const uint8_t*)vcodes;
@@ -997,10 +1022,12 @@ int zk_attention_q8(const void* q, int q_stride, const void* kcodes, const void*
   ZK_REQUIRE(softcap >= 0.f, "zk_attention_q8: softcap must not be negative");
   if (R == 0) return 0;
   ZK_REQUIRE(q && out && ctx_len && (block_table || max_ctx == 0), "zk_attention_q8: null argument");
+  if (window >= max_ctx) window = 0;                   // (sums of ctx and window stay in 32 bits)
   Q8Attention p;
   p.chunk = q8_chunk((long long)max_blocks * bs);
   const int splits = q8_splits(max_ctx, window, p.chunk), blocks = q8_blocks(hd);
   const size_t row = (size_t)R * nh * splits;
+  ZK_REQUIRE(splits <= 65535, "zk_attention_q8: contexts of too many chunks");
   if (splits > 1) {
     ZK_REQUIRE(workspace && (uintptr_t)workspace % 16 == 0, "zk_attention_q8: no workspace, or not at a multiple of 16");
     ZK_REQUIRE(workspace_bytes >= row * (blocks * Q8_BLOCK + 2) * sizeof(float), "zk_attention_q8: the workspace is too small");
@@ -1025,16 +1052,17 @@ int zk_attention_q8(const void* q, int q_stride, const void* kcodes, const void*
   p.window = window;
   // queries by loads of eight, where heads and rows are whole such pieces
   p.q_whole = hd % 8 == 0 && q_stride % 8 == 0 && (uintptr_t)q % (8 * sizeof(act_t)) == 0;
-  const float log2e = 1.44269504088896f;
-  p.k1 = scale * log2e;
+  const double log2e = 1.4426950408889634;
+  p.k1 = (float)(scale * log2e);
 #if ZSE_ACT_BF16
-  p.k2 = softcap > 0.f ? 2.f * scale / softcap * log2e : 0.f;
+  p.k2 = softcap > 0.f ? (float)(2.0 * scale / softcap * log2e) : 0.f;
 #else
   p.k2 = softcap > 0.f ? scale / softcap : 0.f;
 #endif
-  p.c2 = softcap * log2e;
+  p.c2 = (float)(softcap * log2e);
+  p.rest = softcap > 0.f ? (float)(softcap * log2e - p.c2) : (float)(scale * log2e - p.k1);
   const int group = nh / nkv, tiles = (group + 15) / 16;
-  const dim3 grid(splits, nkv * tiles, R);
+  const dim3 grid(nkv * tiles, R, splits);
   // codes past the caches where one block alone reads them and the launch may pass through more than the memory side's cache holds
   const bool once = tiles == 1 && (double)R * max_ctx * nkv * (2 * blocks * Q8_BLOCK + 8) > 256.0 * (1 << 20);
   const size_t lds = (size_t)4 * std::min(group, 16) * (blocks * Q8_BLOCK + 4) * sizeof(float);
