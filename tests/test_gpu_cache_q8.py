@@ -351,6 +351,132 @@ def test_wide_tables(rt, dtype, width):
         assert np.array_equal(alone[0], got[2])
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 4, 128), (34, 2, 256)])
+def test_captured_and_on_two_streams(rt, nh, nkv, hd, dtype):
+    """A token written, attended to and its pages read back, recorded into two graphs that share a workspace and replayed in turn with other
+    tokens, lengths and slots, eager calls on the default stream in between: the bits of the eager calls every time."""
+    rng = np.random.default_rng(hd)
+    k = rt.kernels(dtype)
+    bs, form, R, width = 16, 0, 3, 40
+    lens = [600, 17, 300]
+    table, pages = tables(rng, [640] * R, bs, width)
+    c = random_cache(rng, pages, nkv, hd, bs, form)
+    row = (nh + 2 * nkv) * hd
+    inv = rt.upload((10000.0 ** (-np.arange(hd // 2) * 2.0 / hd)).astype(np.float32))
+    TBL = rt.upload(table)
+    WS = rt.zeros((k.zk_attention_q8_workspace(R, nh, hd, 640, width * bs) // 4 + 1,), "float32")
+
+    class State:
+        def __init__(self):
+            self.cache = device_cache(rt, c)
+            self.X, self.Q, self.OUT = (rt.zeros((R, n), dtype) for n in (row, nh * hd, nh * hd))
+            self.POS, self.SL, self.CL = (rt.zeros((R,), "int32") for _ in range(3))
+            self.K, self.V = rt.zeros((pages, nkv, bs, hd), dtype), rt.zeros((pages, nkv, hd, bs), dtype)
+
+        def fill(self, i):
+            r = np.random.default_rng(i)
+            x = rounded(r.standard_normal((R, row)), dtype)
+            ctx = np.array([n + i for n in lens], np.int32)
+            slots = np.array([table[j, (n - 1) // bs] * bs + (n - 1) % bs for j, n in enumerate(ctx)], np.int32)
+            from zse_amd.weights.safetensors import f32_to_bf16_bits
+            rt.copy_h2d(self.X.ptr, f32_to_bf16_bits(x) if dtype == "bfloat16" else x)
+            for t, a in ((self.POS, ctx - 1), (self.SL, slots), (self.CL, ctx)):
+                rt.copy_h2d(t.ptr, a.astype(np.int32))
+
+        def run(self, stream):
+            kc, vc, sc = self.cache
+            k.zk_rope_cache_write_q8(self.X.ptr, row, None, 0, self.Q.ptr, nh * hd, self.POS.ptr, self.SL.ptr, inv.ptr, hd, kc.ptr, vc.ptr, sc.ptr,
+                                     R, nh, nkv, hd, bs, pages, form, stream)
+            k.zk_attention_q8(self.Q.ptr, nh * hd, kc.ptr, vc.ptr, sc.ptr, TBL.ptr, width, self.CL.ptr, self.OUT.ptr, R, 640, nh, nkv, hd, bs, pages,
+                              0.1, 0.0, 0, form, WS.ptr, WS.nbytes, stream)
+            k.zk_cache_read_q8(kc.ptr, vc.ptr, sc.ptr, TBL.ptr, width, None, self.CL.ptr, self.K.ptr, self.V.ptr, R, 640, 33, nkv, hd, bs, pages, 1,
+                               form, stream)
+
+        def results(self):
+            return [rt.download(t) for t in (*self.cache, self.Q, self.OUT, self.K, self.V)]
+
+    a, b, eager = State(), State(), State()
+    graphs = []
+    for s in (a, b):
+        s.fill(0)
+        s.run(rt.stream)                  # once outside: what a first call sets up is not recorded
+        rt.sync()
+        rt.capture_begin()
+        try:
+            s.run(rt.stream)
+        finally:
+            graphs.append(rt.capture_end())
+    eager.fill(0)
+    eager.run(None)
+    rt._check(rt.lib.zrt_device_sync(), "device sync")
+    for i in range(1, 5):
+        for s, g in ((a, graphs[0]), (b, graphs[1])):
+            s.fill(i)
+            rt.graph_launch(g)
+        rt.sync()
+        eager.fill(i)
+        eager.run(None)
+        rt._check(rt.lib.zrt_device_sync(), "device sync")
+        want = eager.results()
+        for s in (a, b):
+            assert all(np.array_equal(x, y) for x, y in zip(s.results(), want)), i
+    for g in graphs:
+        rt.graph_destroy(g)
+
+
+@pytest.mark.parametrize("nkv,bs", [(2, 16), (1, 64)])
+def test_more_than_64_requests(rt, nkv, bs):
+    """Pages numbered through 150 requests, most of them short, some empty; windows; the attention of all of them."""
+    rng = np.random.default_rng(bs)
+    nh, hd, form, dtype = 4, 64, 1, "bfloat16"
+    k = rt.kernels(dtype)
+    lens = [int(n) for n in rng.integers(0, 90, 150)]
+    lens[::7] = [0] * len(lens[::7])
+    new = [int(rng.integers(0, n + 1)) for n in lens]
+    table, pages = tables(rng, lens, bs, 8)
+    c = random_cache(rng, pages, nkv, hd, bs, form)
+    KC, VC, SC = device_cache(rt, c)
+    TBL, CL, QS = rt.upload(table), rt.upload(np.array(lens, np.int32)), rt.upload(np.cumsum([0] + new).astype(np.int32))
+    for window in (0, 20):
+        K, V = up(rt, np.full((pages, nkv, bs, hd), 3.0), dtype), up(rt, np.full((pages, nkv, bs, hd), 3.0), dtype)
+        k.zk_cache_read_q8(KC.ptr, VC.ptr, SC.ptr, TBL.ptr, 8, QS.ptr, CL.ptr, K.ptr, V.ptr, len(lens), 96, window, nkv, hd, bs, pages, 0, form,
+                           rt.stream)
+        want = np.full((2, pages, nkv, bs, hd), 3.0, np.float32)
+        for r, n in enumerate(lens):
+            for j in range(max(0, n - new[r] + 1 - window) // bs if window else 0, -(-n // bs)):
+                want[:, table[r, j]] = 0.0
+                for t in range(min(bs, n - j * bs)):
+                    for h in range(nkv):
+                        for values in (0, 1):
+                            want[values, table[r, j], h, t] = c.row(table[r, j], h, t, bool(values)).astype(np.float32)
+        assert np.array_equal(rt.download_f32(K), rounded(want[0], dtype)) and np.array_equal(rt.download_f32(V), rounded(want[1], dtype)), window
+        q = rounded(rng.standard_normal((len(lens), nh, hd)), dtype)
+        got = attend(rt, dtype, c, q, table, lens, 96, nh, 0.125, 0.0, window)
+        check_attended(c, got, q, table, lens, nh, 0.125, 0.0, window, dtype)
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 300, 511, 512])
+def test_windows_as_long_as_everything(rt, window):
+    """A window that hides nothing, up to the largest number: the bits of none."""
+    rng = np.random.default_rng(0)
+    nh, nkv, hd, bs, form, dtype = 4, 2, 64, 16, 0, "float32"
+    k = rt.kernels(dtype)
+    lens, new = [500, 1, 0, 40], [7, 1, 0, 40]
+    table, pages = tables(rng, lens, bs, 32)
+    c = random_cache(rng, pages, nkv, hd, bs, form)
+    q = rounded(rng.standard_normal((4, nh, hd)), dtype)
+    assert np.array_equal(*(attend(rt, dtype, c, q, table, lens, 512, nh, 0.125, 0.0, w) for w in (0, window)))
+    KC, VC, SC = device_cache(rt, c)
+    TBL, CL, QS = rt.upload(table), rt.upload(np.array(lens, np.int32)), rt.upload(np.cumsum([0] + new).astype(np.int32))
+    got = []
+    for w in (0, window):
+        K, V = up(rt, np.full((pages, nkv, bs, hd), 3.0), dtype), up(rt, np.full((pages, nkv, bs, hd), 3.0), dtype)
+        k.zk_cache_read_q8(KC.ptr, VC.ptr, SC.ptr, TBL.ptr, 32, QS.ptr, CL.ptr, K.ptr, V.ptr, 4, 512, w, nkv, hd, bs, pages, 0, form, rt.stream)
+        got.append((rt.download(K), rt.download(V)))
+    assert all(np.array_equal(x, y) for x, y in zip(*got))
+
+
 def test_offsets_past_32_bits(rt):
     """A page whose codes lie more than 4 GiB behind the first."""
     nkv, hd, bs, form, nh = 32, 256, 128, 0, 32

@@ -205,6 +205,80 @@ def test_generate(tiny_folders, dtype, cache_dtype):
     assert same >= 0.5 * 20 * len(prompts)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_other_plans(dtype):
+    """Layers with a state beside layers with pages, a layer that reads another entry's keys through a window of its own, queries and keys
+    without positions, a soft cap, and a mixer with a step of its own before the rotation."""
+    import toy_kernels  # noqa: F401  (registers zk_toy_head_norm)
+    from zse_amd.config import (AttentionSpec, BlockSpec, EmbeddingSpec, GatedMLPSpec, HeadSpec, LayerCall, ModelPlan, NormSpec, RotarySpec)
+    from zse_amd.config.plan import NoPositionSpec
+    from zse_amd.engine.loading import random_model
+    from zse_amd.engine.runner import StepEntry, StepRunner
+    from zse_amd.parts.attention import PagedAttention
+    from zse_amd.parts.base import register_part, unregister_part
+    from zse_amd.runtime.device import Runtime
+    from toy_state import DecaySpec, toy_architecture
+    from dataclasses import dataclass
+    rt = Runtime.get()
+    H, V, nh, nkv, hd = 64, 200, 4, 2, 48
+
+    class UnitLengthAttention(PagedAttention):
+        def between_product_and_rotation(self, ctx, qkv):
+            s = self.spec
+            ctx.rt.kernels(ctx.dtype).zk_toy_head_norm(qkv.ptr, qkv.shape[0], qkv.shape[1], s.num_heads + s.num_kv_heads, s.head_dim, ctx.stream)
+
+    @dataclass(frozen=True)
+    class UnitSpec(AttentionSpec):
+        kind: str = "toy_unit_attention"
+
+    def plan_of(cfg):
+        norm = lambda n: NormSpec(H, 1e-6, False, n)
+        names = lambda l, roles: {r: f"l{l}.attn.{r}" for r in roles}
+        rotary = RotarySpec(hd, hd // 2, 1000.0)
+        mixers = [AttentionSpec(H, nh, nkv, hd, 0.3, None, None, rotary, names(0, "qkvo")),
+                  AttentionSpec(H, nh, nkv, hd, 0.3, 5.0, 20, rotary, names(1, "qo")),
+                  DecaySpec(H, 0.75, "l2.mix.w"),
+                  AttentionSpec(H, nh, 1, hd, 0.2, None, 24, NoPositionSpec(), names(3, "qkvo")),
+                  UnitSpec(H, nh, nkv, 32, 2.0, None, None, RotarySpec(32, 32, 1000.0), names(4, "qkvo"))]
+        layers = tuple(BlockSpec("prenorm", m, GatedMLPSpec(H, 96, "silu", {r: f"l{l}.ffn.{r}" for r in ("gate", "up", "down")}),
+                                 {"pre_mixer": norm(f"l{l}.n1"), "pre_ffn": norm(f"l{l}.n2")}) for l, m in enumerate(mixers))
+        return ModelPlan("ToyEightBitLM", H, V, 512, EmbeddingSpec(V, H, 1.0, "emb"), layers,
+                         tuple(LayerCall(l, cache_of=0 if l == 1 else None) for l in range(5)), norm("final"), HeadSpec(V, H, None, "emb"))
+
+    register_part("mixer", "toy_unit_attention", UnitLengthAttention)
+    try:
+        with toy_architecture("ToyEightBitLM", plan_of):
+            model = random_model({"architectures": ["ToyEightBitLM"]}, dtype, seed=4, std=0.1, gain_std=0.1, rt=rt, std_of={"emb": 0.3})
+            rng = np.random.default_rng(0)
+            tokens, other = rng.integers(0, V, 70).tolist(), rng.integers(0, V, 90).tolist()
+
+            def run(cache_dtype, cuts):
+                runner = StepRunner(model, rt, dtype, page_size=16, cache_tokens=512, max_seqs=3, max_batch_tokens=128, max_model_len=256,
+                                    cache_dtype=cache_dtype)
+                rows, at = [], 0
+                for i, n in enumerate(cuts):
+                    z = runner.step([StepEntry("o", other[i:i + 1], []), StepEntry("r", tokens[at:at + n], list(range(n)))])
+                    rows.append(z)
+                    at += n
+                runner.close()
+                return np.concatenate(rows)
+
+            plain = run(None, [70])
+            for cache_dtype in FORMATS:
+                whole, single, mixed = (run(cache_dtype, c) for c in ([70], [1] * 70, [30, 1, 1, 20, 18]))
+                rounding = np.abs(whole - plain).max()
+                # codes are a few hundredths of a value apart: the logits move, and by less than they are large
+                assert 0 < rounding < 0.3 * np.abs(plain).max()
+                for cut in (single, mixed):
+                    err = np.abs(cut - whole)
+                    if dtype == "float32":        # (as in the test of steps of every kind)
+                        assert err.max() < rounding / 4 + F32_ATOL and np.median(err) < F32_ATOL, (cache_dtype, err.max(), rounding)
+                    else:
+                        assert err.max() < BF16_REL * np.abs(plain).max() + 2 * rounding, (cache_dtype, err.max(), rounding)
+    finally:
+        unregister_part("mixer", "toy_unit_attention")
+
+
 def test_refused(tiny_folders):
     from zse_amd.engine.engine import Engine
     with pytest.raises(ValueError, match="16, 32"):
