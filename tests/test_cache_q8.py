@@ -16,11 +16,11 @@ def k(request):
 
 A = 4096            # an address that is never read: every call below ends before a launch
 
-WRITE = dict(qkv=A, ld=2048, planes=None, sums=0, q_out=A, ldq=1024, positions=A, slot_map=A, inv_freq=A, rotary_dim=128, kcodes=A, vcodes=A,
+WRITE = dict(qkv=A, ld=2048, planes=None, sums=0, q_out=A, ldq=2048, positions=A, slot_map=A, inv_freq=A, rotary_dim=128, kcodes=A, vcodes=A,
              scales=A, T=3, nh=8, nkv=4, hd=128, bs=16, num_pages=9, format=0, stream=None)
 READ = dict(kcodes=A, vcodes=A, scales=A, block_table=A, max_blocks=8, q_start=None, ctx_len=A, k=A, v=A, R=2, max_ctx=128, window=0, nkv=4, hd=128,
             bs=16, num_pages=9, v_transposed=1, format=1, stream=None)
-ATTEND = dict(q=A, q_stride=1024, kcodes=A, vcodes=A, scales=A, block_table=A, max_blocks=8, ctx_len=A, out=A, R=2, max_ctx=128, nh=8, nkv=4, hd=128,
+ATTEND = dict(q=A, q_stride=1024, kcodes=A, vcodes=A, scales=A, block_table=A, max_blocks=8, ctx_len=A, out=1 << 30, R=2, max_ctx=128, nh=8, nkv=4, hd=128,
               bs=16, num_pages=9, scale=0.1, softcap=0.0, window=0, format=0, workspace=A, workspace_bytes=1 << 30, stream=None)
 
 CACHE = [(dict(bs=8), "pages of 16"), (dict(bs=0), "pages of 16"), (dict(bs=24), "pages of 16"), (dict(num_pages=0), "one page"),
@@ -32,7 +32,8 @@ CACHE = [(dict(bs=8), "pages of 16"), (dict(bs=0), "pages of 16"), (dict(bs=24),
     (dict(T=-1), "bad sizes"), (dict(nh=0), "bad sizes"), (dict(nkv=-1), "bad sizes"), (dict(sums=-1), "bad sizes"), (dict(nkv=20000), "too many"),
     (dict(rotary_dim=3), "even"), (dict(rotary_dim=130), "at most"), (dict(inv_freq=None), "frequency"), (dict(ld=2047), "overlap"),
     (dict(ldq=1023), "overlap"), (dict(qkv=None), "null"), (dict(q_out=None), "null"), (dict(positions=None), "null"),
-    (dict(sums=2, planes=None), "null"), (dict(sums=2, planes=A + 4), "misaligned")])
+    (dict(sums=2, planes=None), "null"), (dict(sums=2, planes=A + 4), "misaligned"),
+    (dict(ldq=1024, q_out=A), "where they came from"), (dict(q_out=A + 64, ldq=2048), "where they came from")])
 def test_write_refuses(k, change, says):
     from zse_amd.runtime.device import DeviceError
     with pytest.raises(DeviceError, match=f"zk_rope_cache_write_q8.*{says}"):
@@ -41,7 +42,7 @@ def test_write_refuses(k, change, says):
 
 @pytest.mark.parametrize("change,says", CACHE + [
     (dict(R=-1), "bad sizes"), (dict(max_ctx=-1), "bad sizes"), (dict(window=-1), "bad sizes"), (dict(max_ctx=129), "longer than the table"),
-    (dict(nkv=0), ""), (dict(nkv=70000), "too many"), (dict(R=70000), "too many"), (dict(block_table=None), "null"), (dict(ctx_len=None), "null"),
+    (dict(max_ctx=2 ** 30 + 1, max_blocks=2 ** 30), "2\\^30"), (dict(nkv=0), ""), (dict(nkv=70000), "too many"), (dict(R=70000), "too many"), (dict(block_table=None), "null"), (dict(ctx_len=None), "null"),
     (dict(k=None), "null"), (dict(v=A + 8), "misaligned")])
 def test_read_refuses(k, change, says):
     from zse_amd.runtime.device import DeviceError
@@ -54,7 +55,8 @@ def test_read_refuses(k, change, says):
     (dict(nh=9), "multiple"), (dict(q_stride=1023), "overlap"), (dict(nh=70000, q_stride=70000 * 128), "too many"),
     (dict(max_ctx=129), "longer than the table"), (dict(softcap=-1.0), "softcap"), (dict(q=None), "null"), (dict(out=None), "null"),
     (dict(ctx_len=None), "null"), (dict(block_table=None), "null"), (dict(R=70000), "too many"), (dict(num_pages=1 << 30), "too many pages"),
-    (dict(max_ctx=20000, max_blocks=2000, workspace=None), "no workspace"), (dict(max_ctx=20000, max_blocks=2000, workspace=A + 4), "multiple of 16"),
+    (dict(max_ctx=2 ** 30 + 1, max_blocks=2 ** 30), "2\\^30"), (dict(max_ctx=2 ** 30, max_blocks=2 ** 30), "too many chunks"),
+    (dict(out=A + 2 * 1024), "results over queries"), (dict(max_ctx=20000, max_blocks=2000, workspace=None), "no workspace"), (dict(max_ctx=20000, max_blocks=2000, workspace=A + 4), "multiple of 16"),
     (dict(max_ctx=20000, max_blocks=2000, workspace_bytes=1000), "too small")])
 def test_attention_refuses(k, change, says):
     from zse_amd.runtime.device import DeviceError

@@ -40,6 +40,7 @@ __device__ __forceinline__ size_t q8_scale(int page, int head, int nkv, int bs, 
 
 template <int FMT>
 __device__ __forceinline__ float q8_top() { return FMT == 0 ? 127.f : 448.f; }
+
 // Four values times ``factor`` as four codes.  |x| factor is at most top and a rounding, which the nearest code of either kind is top
 // for: nothing has to be cut off.
 template <int FMT>
@@ -74,6 +75,7 @@ __device__ __forceinline__ void q8_scales(float a, float& scale, float& factor) 
     factor = __fdiv_rn(top, a);
   }
 }
+
 // Sine and cosine of pos * freq, positions below 2^24.  The product is held in two floats (rounded to one it is off by up to half
 // a step of the angle, 2^-12 at position 4,096 and 2^-7 at 131,072), less whole quarters of a turn (pi / 2 in two floats; n times the
 // first takes nothing from a multiple of its last place), then one float r and what that leaves, which turns the result to first
@@ -103,7 +105,6 @@ typedef unsigned q8_u4 __attribute__((ext_vector_type(4)));
 typedef act_t q8_a4 __attribute__((ext_vector_type(4)));
 #if ZSE_ACT_BF16
 typedef __bf16 q8_b8 __attribute__((ext_vector_type(8)));
-typedef __bf16 q8_b2 __attribute__((ext_vector_type(2)));
 #endif
 
 // Four codes as four numbers of the type that the products take.
@@ -123,6 +124,7 @@ __device__ __forceinline__ void q8_floats(unsigned codes, float (&x)[4]) {
   }
 #endif
 }
+
 // ---------------------------------------------------------------- written
 // A block takes four rows of the step, a group of LANES lanes a head of them at a time, four neighbouring channels a lane: the
 // head's largest magnitude is a maximum over the group's lanes, and four rows whose slots are four in a row from a multiple of four on
@@ -201,38 +203,33 @@ __global__ __launch_bounds__(256, WHOLE ? 4 : 2) void write_q8_kernel(Q8Write<SU
   const int near = t0 - 3 + lane;
   int slots = p.slot_map && lane < 10 && near >= 0 && near < p.T ? p.slot_map[near] : -1;
   const float position = lane < 10 && near >= 0 && near < p.T ? (float)p.positions[near] : 0.f;
-  if (slots >= 0 && slots / p.bs >= p.num_pages) slots = -1;
+  const int page = slots / p.bs;
+  if (page >= p.num_pages) slots = -1;
+  const int off = slots - page * p.bs;
+  // (what follows is of a slot that is there; of others it is not used)
+  const int piece_of = slots < 0 ? 0 : page * p.nkv * pieces + off / Q8_PIECE, scale_of = slots < 0 ? 0 : page * p.nkv * 2 * p.bs + off;
   const int s1 = __shfl(slots, lane + 1), s2 = __shfl(slots, lane + 2), s3 = __shfl(slots, lane + 3);
   const unsigned fours = (unsigned)__ballot(lane < 7 && slots >= 0 && slots % 4 == 0 && s1 == slots + 1 && s2 == slots + 2 && s3 == slots + 3);
-  const int page = slots >= 0 ? slots / p.bs : 0, off = slots >= 0 ? slots % p.bs : 0;
-  const size_t piece_of = ((size_t)page * p.nkv * pieces + off / Q8_PIECE) * (size_t)(blocks * Q8_BYTES);
-  const size_t scale_of = (size_t)page * p.nkv * 2 * p.bs + off;
-  auto of_row = [](size_t v, int i) {
-    return (size_t)(unsigned)__builtin_amdgcn_readlane((int)v, i) | (size_t)__builtin_amdgcn_readlane((int)(v >> 32), i) << 32;
-  };
   for (int taken = 0; taken < 2; taken++) {
     // the four that begins among the block's rows, then the block's rows that are in none
     const bool four = taken == 0;
-    unsigned mine = 0;                                   // bit t: there is a row t
-    if (four) mine = fours & 0x78 ? 15 : 0;
-    else
-      for (int t = 0; t < 4; t++) mine |= !(fours >> t & 15) && t0 + t < p.T ? 1u << t : 0u;
+    const unsigned held = (1u << min(4, p.T - t0)) - 1;       // the block's rows that there are
+    const unsigned mine = four ? (fours & 0x78 ? 15 : 0)
+                               : held & ~(fours | fours >> 1 | fours >> 2 | fours >> 3);      // bit t: there is a row t
     if (!mine) continue;
-    const int start = four ? __builtin_ctz(fours & 0x78) : 3, present = start + __builtin_ctz(mine);
-    int row[4], slot[4], at[4];                          // what is not there is read as a row that is, and not stored
+    const int start = four ? __builtin_ctz(fours & 0x78) : 3;
+    int row[4], slot[4], at[4];
     size_t piece[4];
 #pragma unroll
     for (int t = 0; t < 4; t++) {
-      const int i = mine >> t & 1 ? start + t : present;
-      row[t] = t0 - 3 + i;
-      slot[t] = mine >> t & 1 ? __builtin_amdgcn_readlane(slots, i) : -1;
-      at[t] = __builtin_amdgcn_readlane(off, i) % Q8_PIECE;
-      piece[t] = of_row(piece_of, i);
+      row[t] = min(t0 - 3 + start + t, p.T - 1);              // (one that is not there is not stored)
+      slot[t] = mine >> t & 1 ? __builtin_amdgcn_readlane(slots, start + t) : -1;
+      at[t] = __builtin_amdgcn_readlane(off, start + t) % Q8_PIECE;
+      piece[t] = (size_t)__builtin_amdgcn_readlane(piece_of, start + t) * (unsigned)(blocks * Q8_BYTES);
     }
     // lane t of every quad: row t's, for its scales
-    const int quad = mine >> (lane & 3) & 1 ? start + (lane & 3) : present;
-    const int quad_slot = mine >> (lane & 3) & 1 ? __shfl(slots, quad) : -1;
-    const size_t quad_scale = (size_t)(unsigned)__shfl((int)scale_of, quad) | (size_t)__shfl((int)(scale_of >> 32), quad) << 32;
+    const int quad_of = __shfl(slots, start + (lane & 3)), quad_scale = __shfl(scale_of, start + (lane & 3));
+    const int quad_slot = mine >> (lane & 3) & 1 ? quad_of : -1;
     const bool stores = slot[0] >= 0 || slot[1] >= 0 || slot[2] >= 0 || slot[3] >= 0;
     bool turned = false;
     const int pass = gridDim.y * HEADS;
@@ -254,7 +251,7 @@ __global__ __launch_bounds__(256, WHOLE ? 4 : 2) void write_q8_kernel(Q8Write<SU
         }
       }
     };
-    if (blockIdx.y * HEADS < p.heads) ask(blockIdx.y * HEADS);
+    ask(blockIdx.y * HEADS);
     for (int base = blockIdx.y * HEADS; base < p.heads; base += pass) {
       const int head = min(base + sub, p.heads - 1);
       const bool live = base + sub < p.heads, is_q = head < p.nh, is_v = head >= p.nh + p.nkv;
@@ -369,7 +366,7 @@ __global__ __launch_bounds__(256, WHOLE ? 4 : 2) void write_q8_kernel(Q8Write<SU
         }
       }
       // the head's first four lanes: a row's scale each
-      if (c0 < 16 && quad_slot >= 0) p.scales[quad_scale + (size_t)(2 * kvh + is_v) * p.bs] = scale;
+      if (c0 < 16 && quad_slot >= 0) p.scales[(unsigned)quad_scale + (size_t)(2 * kvh + is_v) * p.bs] = scale;
     }
   }
 #endif
@@ -865,6 +862,14 @@ static int q8_refuses(const char* who, const void* kcodes, const void* vcodes, c
 }
 #define Q8_REQUIRE_CACHE(who) \
   if (const int rc = q8_refuses(who, kcodes, vcodes, scales, nkv, hd, bs, num_pages, format)) return rc
+
+// Whether two ranges of values of the activations' type meet: ``rows`` rows of ``width``, ``ld`` apart.
+static bool q8_meet(const void* a, long long a_ld, long long a_width, const void* b, long long b_ld, long long b_width, long long rows) {
+  const uintptr_t a0 = (uintptr_t)a, a1 = a0 + ((rows - 1) * a_ld + a_width) * sizeof(act_t);
+  const uintptr_t b0 = (uintptr_t)b, b1 = b0 + ((rows - 1) * b_ld + b_width) * sizeof(act_t);
+  return a0 < b1 && b0 < a1;
+}
+
 // Blocks of a launch.  Written: the heads of four rows are dealt to as many blocks as that gives (4,092 rows of 32 heads and 2 x 16 of
 // 128 channels by 1,024, 2,048 and 4,096 blocks 43, 40 and 38 us; more work out the same angles).  Read back: waves that take
 // pieces in turn (64 pages of 8 heads in a range of 64,512 pieces by 2,048, 4,096 and 8,192 blocks 6.2, 8.1 and 10.4 us, empty ones
@@ -883,6 +888,7 @@ static void q8_by_flag(bool flag, F go) {
   if (flag) go(std::true_type());
   else go(std::false_type());
 }
+
 // Keys of a partial result, by what a request's table can hold.  us by 256, 512 and 1,024 keys (16-bit rows, 8 heads over 4 of 256
 // channels): one request of 4,000 keys 10.8, 12.8, 18.9; 64 of them 98.6, 93.7, 91.4; one of 16,000 15.6, 15.3, 20.8; eight of
 // them 56.3, 49.8, 47.9; one of 60,000 45.1, 33.5, 28.3.  32-bit products take eight times as long for as many keys: by 128, 256
@@ -894,9 +900,10 @@ static int q8_chunk(long long table_tokens) {
   return table_tokens < 8192 ? 128 : 256;
 #endif
 }
+
 // Chunks that a request of up to max_ctx tokens may meet.
 static int q8_splits(int max_ctx, int window, int chunk) {
-  const int all = std::max(1, (max_ctx + chunk - 1) / chunk);
+  const int all = (int)std::max(1ll, ((long long)max_ctx + chunk - 1) / chunk);
   return window > 0 ? (int)std::min<long long>(all, ((long long)window + chunk - 2) / chunk + 1) : all;
 }
 
@@ -919,6 +926,7 @@ int zk_rope_cache_write_q8(const void* qkv, int ld, const float* planes, int sum
   ZK_REQUIRE(hd > 0 && hd <= 256, "zk_rope_cache_write_q8: heads of 1 to 256 channels");
   ZK_REQUIRE(nh <= 16384 && nkv <= 16384, "zk_rope_cache_write_q8: too many heads");
   if (nkv > 0 && slot_map) Q8_REQUIRE_CACHE("zk_rope_cache_write_q8");
+  ZK_REQUIRE(nkv == 0 || !slot_map || (long long)num_pages * nkv * 2 * bs < (1ll << 31), "zk_rope_cache_write_q8: too many pages");
   ZK_REQUIRE(format == 0 || format == 1, "zk_rope_cache_write_q8: format 0 (int8) or 1 (e4m3)");
   ZK_REQUIRE(rotary_dim >= 0 && rotary_dim <= hd && rotary_dim % 2 == 0,
              "zk_rope_cache_write_q8: rotary_dim must be even and at most head_dim");
@@ -929,6 +937,8 @@ int zk_rope_cache_write_q8(const void* qkv, int ld, const float* planes, int sum
              "zk_rope_cache_write_q8: null or misaligned argument");
   const int width = (nh + 2 * nkv) * hd, blocks = q8_blocks(hd);
   const bool partial = sums > 0;
+  ZK_REQUIRE(partial || (q_out == qkv && ldq == ld) || !q8_meet(qkv, ld, width, q_out, ldq, (long long)nh * hd, T),
+             "zk_rope_cache_write_q8: queries may go where they came from, in rows as far apart, or elsewhere");
   const int row = partial ? width : ld, heads = slot_map ? nh + 2 * nkv : nh;
   const bool whole = hd % 4 == 0 && rotary_dim % 8 == 0 && row % 4 == 0 && ldq % 4 == 0 && (uintptr_t)q_out % (4 * sizeof(act_t)) == 0 &&
                      (partial || (uintptr_t)qkv % (4 * sizeof(act_t)) == 0);
@@ -956,12 +966,14 @@ int zk_rope_cache_write_q8(const void* qkv, int ld, const float* planes, int sum
 // Reads the pages back that requests 0 .. R-1 see, into the same pages of k and v [num_pages][nkv][bs][hd] in the activations' type
 // (v_transposed: values as [num_pages][nkv][hd][bs]).  A request of ctx_len[r] tokens, the last q_start[r + 1] - q_start[r] of
 // them new (q_start null: one), sees positions from max(0, ctx - new + 1 - window) on, all without a window.  Slots behind its last
-// token are read as zeros; other pages stay as they were.
+// token are read as zeros; other pages stay as they were.  A page belongs to one request (one that two requests name is read as either
+// of them sees it).
 int zk_cache_read_q8(const void* kcodes, const void* vcodes, const float* scales, const int* block_table, int max_blocks,
                      const int* q_start, const int* ctx_len, void* k, void* v, int R, int max_ctx, int window, int nkv, int hd, int bs,
                      int num_pages, int v_transposed, int format, void* stream) {
   Q8_REQUIRE_CACHE("zk_cache_read_q8");
   ZK_REQUIRE(R >= 0 && max_ctx >= 0 && window >= 0 && max_blocks >= 0, "zk_cache_read_q8: bad sizes");
+  ZK_REQUIRE(max_ctx <= 1 << 30, "zk_cache_read_q8: contexts of more than 2^30 tokens");
   ZK_REQUIRE(max_ctx <= (long long)max_blocks * bs, "zk_cache_read_q8: contexts longer than the table");
   ZK_REQUIRE(nkv <= 65535 && R <= 65535, "zk_cache_read_q8: too many requests or heads");
   if (R == 0 || max_ctx == 0) return 0;
@@ -1007,7 +1019,7 @@ size_t zk_attention_q8_workspace(int R, int nh, int hd, int max_ctx, int table_t
 
 // Attention of one token a request, the last of its ctx_len[r], over its cache: z_j = scale q.k_j (softcap > 0: softcap
 // tanh(z_j / softcap)) for j from max(0, ctx - window) on (all without a window), out = sum softmax(z)_j v_j.  q: row r at r * q_stride;
-// out: rows of nh * hd.  A request without keys gets zeros, and a page that the table does not name (below zero, or not below
+// out: rows of nh * hd, apart from q.  A request without keys gets zeros, and a page that the table does not name (below zero, or not below
 // num_pages) has none.
 int zk_attention_q8(const void* q, int q_stride, const void* kcodes, const void* vcodes, const float* scales, const int* block_table,
                     int max_blocks, const int* ctx_len, void* out, int R, int max_ctx, int nh, int nkv, int hd, int bs, int num_pages,
@@ -1017,11 +1029,13 @@ int zk_attention_q8(const void* q, int q_stride, const void* kcodes, const void*
   ZK_REQUIRE(nh % nkv == 0, "zk_attention_q8: query heads must be a multiple of key heads");
   ZK_REQUIRE(nh <= 65535 && R <= 65535, "zk_attention_q8: too many heads or requests");
   ZK_REQUIRE(q_stride >= (long long)nh * hd, "zk_attention_q8: rows overlap");
+  ZK_REQUIRE(max_ctx <= 1 << 30, "zk_attention_q8: contexts of more than 2^30 tokens");
   ZK_REQUIRE(max_ctx <= (long long)max_blocks * bs, "zk_attention_q8: contexts longer than the table");
   ZK_REQUIRE((long long)num_pages * nkv * 2 * (bs / Q8_PIECE) < (1ll << 31), "zk_attention_q8: too many pages");
   ZK_REQUIRE(softcap >= 0.f, "zk_attention_q8: softcap must not be negative");
   if (R == 0) return 0;
   ZK_REQUIRE(q && out && ctx_len && (block_table || max_ctx == 0), "zk_attention_q8: null argument");
+  ZK_REQUIRE(!q8_meet(q, q_stride, (long long)nh * hd, out, (long long)nh * hd, (long long)nh * hd, R), "zk_attention_q8: results over queries");
   if (window >= max_ctx) window = 0;                   // (sums of ctx and window stay in 32 bits)
   Q8Attention p;
   p.chunk = q8_chunk((long long)max_blocks * bs);
