@@ -38,6 +38,11 @@ __device__ __forceinline__ size_t q8_scale(int page, int head, int nkv, int bs, 
   return (((size_t)page * nkv + head) * 2 + values) * (size_t)bs;
 }
 
+// x / n; ``shift``: where n is a power of two its exponent, else -1 (a division is some thirty instructions, and a kernel of few
+// blocks is as long as one wave's chain of them).
+__device__ __forceinline__ int q8_div(int x, int n, int shift) { return shift >= 0 ? x >> shift : x / n; }
+static int q8_shift(int n) { return (n & (n - 1)) == 0 ? __builtin_ctz(n) : -1; }
+
 template <int FMT>
 __device__ __forceinline__ float q8_top() { return FMT == 0 ? 127.f : 448.f; }
 
@@ -162,7 +167,7 @@ struct Q8Write {
   const float* inv_freq;
   uint8_t *kcodes, *vcodes;
   float* scales;
-  int ldq, rotary_dim, T, nh, nkv, hd, bs, num_pages, heads;
+  int ldq, rotary_dim, T, nh, nkv, hd, bs, bs_shift, num_pages, heads;
 };
 
 // The largest of a group of 16, 32 or 64 lanes' magnitudes as bits (a NaN is larger than infinity, and that than any number).
@@ -203,7 +208,7 @@ __global__ __launch_bounds__(256, WHOLE ? 4 : 2) void write_q8_kernel(Q8Write<SU
   const int near = t0 - 3 + lane;
   int slots = p.slot_map && lane < 10 && near >= 0 && near < p.T ? p.slot_map[near] : -1;
   const float position = lane < 10 && near >= 0 && near < p.T ? (float)p.positions[near] : 0.f;
-  const int page = slots / p.bs;
+  const int page = q8_div(slots, p.bs, p.bs_shift);
   if (page >= p.num_pages) slots = -1;
   const int off = slots - page * p.bs;
   // (what follows is of a slot that is there; of others it is not used)
@@ -380,7 +385,7 @@ struct Q8Read {
   const float* scales;
   const int *block_table, *q_start, *ctx_len;
   act_t *k, *v;
-  int R, max_blocks, max_ctx, window, nkv, hd, bs, num_pages;
+  int R, max_blocks, max_ctx, window, nkv, hd, bs, bs_shift, num_pages;
 };
 
 template <int FMT, bool TRANSPOSED, bool WHOLE>
@@ -389,18 +394,20 @@ __global__ __launch_bounds__(256) void read_q8_kernel(Q8Read p) {
   typedef unsigned u2 __attribute__((ext_vector_type(2)));
   typedef q8_a4 a4;
   typedef act_t a8 __attribute__((ext_vector_type(8)));
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pieces = p.bs / Q8_PIECE, per_page = pieces * p.nkv;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pieces = p.bs / Q8_PIECE;
+  const int per_page = pieces * p.nkv;
   // the requests' pages are numbered through, 64 requests at a time: lane i knows where those of request r0 + i end
   int r0 = -64, before = 0, upto = 0, ends = 0, ctx_of = 0, first_of = 0;      // before, upto: of the 64 requests' pages
   for (int item = blockIdx.x * 4 + wave;; item += gridDim.x * 4) {
-    const int x = item / per_page, rest = item % per_page, head = rest / pieces, sub = rest % pieces;
+    const int x = item / per_page, rest = item - x * per_page;
+    const int head = q8_div(rest, pieces, p.bs_shift >= 0 ? p.bs_shift - 4 : -1), sub = rest - head * pieces;
     while (x >= upto) {
       r0 += 64;
       if (r0 >= p.R) return;
       const int r = min(r0 + lane, p.R - 1), ctx = min(p.ctx_len[r], p.max_ctx), rows = p.q_start ? p.q_start[r + 1] - p.q_start[r] : 1;
       ctx_of = ctx;
-      first_of = (p.window > 0 ? max(0, ctx - rows + 1 - p.window) : 0) / p.bs;
-      ends = upto + wave_running_sum(r0 + lane < p.R ? max(0, (ctx + p.bs - 1) / p.bs - first_of) : 0);
+      first_of = q8_div(p.window > 0 ? max(0, ctx - rows + 1 - p.window) : 0, p.bs, p.bs_shift);
+      ends = upto + wave_running_sum(r0 + lane < p.R ? max(0, q8_div(max(ctx, 0) + p.bs - 1, p.bs, p.bs_shift) - first_of) : 0);
       before = upto;
       upto = __builtin_amdgcn_readlane(ends, 63);
     }
@@ -476,7 +483,7 @@ struct Q8Attention {
   const int *block_table, *ctx_len;
   act_t* out;
   float *part_o, *part_ml;          // [R][nh][splits][channels, filled up] and [..][2]
-  int q_stride, max_blocks, max_ctx, nh, nkv, hd, pieces, num_pages, window, chunk, q_whole;
+  int q_stride, max_blocks, max_ctx, nh, nkv, hd, pieces, pieces_shift, num_pages, window, chunk, chunk_shift, q_whole;
   float k1, k2, c2;                 // z log2(e) = k1 dot, or c2 tanh(k2 dot)
   float rest;                       // what k1, or c2, is short of its value
 };
@@ -523,9 +530,9 @@ __global__ __launch_bounds__(256, 2) void attention_q8_kernel(Q8Attention p) {
   const int group = p.nh / p.nkv, kvh = blockIdx.x % p.nkv, head0 = blockIdx.x / p.nkv * 16, heads = min(16, group - head0);
   // without a window the chunk's place in the table does not wait for the request's length
   int early = -1;
-  if (p.window == 0 && p.max_ctx > 0) early = p.block_table[(size_t)r * p.max_blocks + min((split * (p.chunk / Q8_PIECE) + lane) / p.pieces, p.max_blocks - 1)];
+  if (p.window == 0 && p.max_ctx > 0) early = p.block_table[(size_t)r * p.max_blocks + min(q8_div(split * (p.chunk / Q8_PIECE) + lane, p.pieces, p.pieces_shift), p.max_blocks - 1)];
   const int ctx = min(p.ctx_len[r], p.max_ctx), first = p.window > 0 ? max(0, ctx - p.window) : 0;
-  const int from = first / p.chunk * p.chunk + split * p.chunk;
+  const int from = ((first >> p.chunk_shift) + split) << p.chunk_shift;
   const int begin = max(first, from), end = min(ctx, from + p.chunk);
   const int head = kvh * group + head0 + col;             // this lane's column, if col < heads
   if (begin >= end) {
@@ -538,11 +545,12 @@ __global__ __launch_bounds__(256, 2) void attention_q8_kernel(Q8Attention p) {
   const int p0 = begin / Q8_PIECE, n_pieces = (end + Q8_PIECE - 1) / Q8_PIECE - p0;
   int piece_at = -1, scale_at = 0;
   if (lane < n_pieces) {
-    const int i = p0 + lane, page = p.window == 0 ? early : p.block_table[(size_t)r * p.max_blocks + i / p.pieces];
+    const int i = p0 + lane, of = q8_div(i, p.pieces, p.pieces_shift), sub = i - of * p.pieces;
+    const int page = p.window == 0 ? early : p.block_table[(size_t)r * p.max_blocks + of];
     if (page >= 0 && page < p.num_pages) {
       const int at = page * p.nkv + kvh;
-      piece_at = at * p.pieces + i % p.pieces;
-      scale_at = at * 2 * p.pieces + i % p.pieces;
+      piece_at = at * p.pieces + sub;
+      scale_at = at * 2 * p.pieces + sub;
     }
   }
   const int n_pairs = (n_pieces + 1) / 2;
@@ -809,7 +817,7 @@ __global__ __launch_bounds__(256) void attention_q8_join_kernel(Q8Attention p, i
   q8_f4 x[AHEAD];
 #pragma unroll
   for (int e = 0; e < AHEAD; e++) x[e] = *(const q8_f4*)(part + (size_t)min(group + e * GROUPS, splits - 1) * (NB * 64));
-  const int n = ctx > 0 ? (ctx + p.chunk - 1) / p.chunk - first / p.chunk : 0;
+  const int n = ctx > 0 ? ((ctx + p.chunk - 1) >> p.chunk_shift) - (first >> p.chunk_shift) : 0;
   float most = lane < n ? mine[0] : -INFINITY;
   for (int i = lane + 64; i < n; i += 64) most = fmaxf(most, ml[i][0]);
   most = wave_max_whole(most);
@@ -947,7 +955,7 @@ int zk_rope_cache_write_q8(const void* qkv, int ld, const float* planes, int sum
   auto launch = [&](auto format_of, auto lanes_of, auto whole_of, auto partial_of) {
     constexpr bool SUMS = decltype(partial_of)::value;
     const Q8Write<SUMS> p{{(const act_t*)qkv, planes, row, sums, (size_t)T * width}, (act_t*)q_out, positions, slot_map, inv_freq,
-                          (uint8_t*)kcodes, (uint8_t*)vcodes, (float*)scales, ldq, rotary_dim, T, nh, nkv, hd, bs, num_pages, heads};
+                          (uint8_t*)kcodes, (uint8_t*)vcodes, (float*)scales, ldq, rotary_dim, T, nh, nkv, hd, bs, q8_shift(bs), num_pages, heads};
     write_q8_kernel<decltype(format_of)::value, decltype(lanes_of)::value, decltype(whole_of)::value, SUMS>
         <<<grid, 256, 0, (hipStream_t)stream>>>(p);
   };
@@ -994,10 +1002,11 @@ int zk_cache_read_q8(const void* kcodes, const void* vcodes, const float* scales
   p.nkv = nkv;
   p.hd = hd;
   p.bs = bs;
+  p.bs_shift = q8_shift(bs);
   p.num_pages = num_pages;
   p.R = R;
   // how much of it the requests' windows cover is not known here: blocks enough to fill the chip, whose waves take pieces in turn
-  const long long pieces = (long long)((max_ctx + bs - 1) / bs) * (bs / Q8_PIECE) * nkv * R;
+  const long long pieces = ((max_ctx + (long long)bs - 1) / bs) * (bs / Q8_PIECE) * nkv * R;
   ZK_REQUIRE(pieces < (1ll << 30), "zk_cache_read_q8: too many pages");
   const int grid = (int)std::min<long long>((pieces + 3) / 4, Q8_READ_BLOCKS);
   q8_by_format(format, [&](auto f) {
@@ -1062,6 +1071,8 @@ int zk_attention_q8(const void* q, int q_stride, const void* kcodes, const void*
   p.nkv = nkv;
   p.hd = hd;
   p.pieces = bs / Q8_PIECE;
+  p.pieces_shift = q8_shift(p.pieces);
+  p.chunk_shift = q8_shift(p.chunk);
   p.num_pages = num_pages;
   p.window = window;
   // queries by loads of eight, where heads and rows are whole such pieces
