@@ -108,6 +108,7 @@ __device__ __forceinline__ void q8_sincos(float pos, float freq, float& sn, floa
 typedef float q8_f4 __attribute__((ext_vector_type(4)));
 typedef unsigned q8_u4 __attribute__((ext_vector_type(4)));
 typedef act_t q8_a4 __attribute__((ext_vector_type(4)));
+typedef act_t q8_a8 __attribute__((ext_vector_type(8)));
 #if ZSE_ACT_BF16
 typedef __bf16 q8_b8 __attribute__((ext_vector_type(8)));
 #endif
@@ -378,8 +379,10 @@ __global__ __launch_bounds__(256, WHOLE ? 4 : 2) void write_q8_kernel(Q8Write<SU
 }
 
 // ---------------------------------------------------------------- read back
-// A wave reads a piece of one head: keys eight channels a lane, so that a load is 512 bytes in a row and a store whole rows of 64
-// channels; values as the layout has them, four neighbouring tokens of four channels a lane.
+// A wave reads a piece of one head, or two neighbouring ones (PAIRS: pages of an even number of pieces): keys eight channels a lane, so
+// that a load is 512 bytes in a row and a store whole rows of 64 channels; values as the layout has them, four neighbouring tokens of
+// four channels a lane.  Where they go out transposed in 16 bits, rows of 16 lanes exchange words, and a lane stores eight neighbouring
+// tokens of a channel: with pairs a store is 16 channels' runs of 64 bytes.
 struct Q8Read {
   const uint8_t *kcodes, *vcodes;
   const float* scales;
@@ -388,19 +391,18 @@ struct Q8Read {
   int R, max_blocks, max_ctx, window, nkv, hd, bs, bs_shift, num_pages;
 };
 
-template <int FMT, bool TRANSPOSED, bool WHOLE>
+template <int FMT, bool TRANSPOSED, bool WHOLE, bool PAIRS>
 __global__ __launch_bounds__(256) void read_q8_kernel(Q8Read p) {
 #ifdef __HIP_DEVICE_COMPILE__
   typedef unsigned u2 __attribute__((ext_vector_type(2)));
-  typedef q8_a4 a4;
-  typedef act_t a8 __attribute__((ext_vector_type(8)));
+  constexpr int U = PAIRS ? 2 : 1;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pieces = p.bs / Q8_PIECE;
-  const int per_page = pieces * p.nkv;
+  const int turns = pieces / U, turns_shift = p.bs_shift >= 0 ? p.bs_shift - 4 - (U - 1) : -1, per_page = turns * p.nkv;
   // the requests' pages are numbered through, 64 requests at a time: lane i knows where those of request r0 + i end
   int r0 = -64, before = 0, upto = 0, ends = 0, ctx_of = 0, first_of = 0;      // before, upto: of the 64 requests' pages
   for (int item = blockIdx.x * 4 + wave;; item += gridDim.x * 4) {
     const int x = item / per_page, rest = item - x * per_page;
-    const int head = q8_div(rest, pieces, p.bs_shift >= 0 ? p.bs_shift - 4 : -1), sub = rest - head * pieces;
+    const int head = q8_div(rest, turns, turns_shift), sub = (rest - head * turns) * U;
     while (x >= upto) {
       r0 += 64;
       if (r0 >= p.R) return;
@@ -420,45 +422,73 @@ __global__ __launch_bounds__(256) void read_q8_kernel(Q8Read p) {
     const size_t at = q8_piece(page, sub, head, p.nkv, pieces, blocks);
     const float* scales = p.scales + q8_scale(page, head, p.nkv, p.bs, 0) + sub * Q8_PIECE;
     const size_t out = ((size_t)page * p.nkv + head) * (size_t)(p.bs * p.hd);
-    const int t0 = lane / 8, c8 = lane % 8 * 8;
-    const float ks[2] = {scales[t0], scales[t0 + 8]};
-    const q8_f4 vs = *(const q8_f4*)(scales + p.bs + lane / 16 * 4);
+    const int t0 = lane / 8, c8 = lane % 8 * 8, row = lane / 16, col = lane % 16;
+    float ks[2 * U];
+#pragma unroll
+    for (int u = 0; u < 2 * U; u++) ks[u] = scales[t0 + 8 * u];
+    constexpr bool EIGHTS = TRANSPOSED && sizeof(act_t) == 2;
+    static_assert(EIGHTS || !PAIRS, "pairs of pieces go out by eights");
+    // the tokens that a lane stores of a channel: eight from ``first``, or four
+    const int first = PAIRS ? (row & 1) * 16 + row / 2 * 8 : row / 2 * 8;
+    q8_f4 vs[2];
+    vs[0] = *(const q8_f4*)(scales + p.bs + (EIGHTS ? first : row * 4));
+    vs[1] = *(const q8_f4*)(scales + p.bs + (EIGHTS ? first + 4 : row * 4));
     for (int n = 0; n < blocks; n++) {
-      u2 kw[2];
+      u2 kw[2 * U];
+      q8_u4 vw[U];
 #pragma unroll
-      for (int u = 0; u < 2; u++) kw[u] = *(const u2*)(p.kcodes + at + n * Q8_BYTES + u * 512 + lane * 8);
-      const q8_u4 vw = *(const q8_u4*)(p.vcodes + at + n * Q8_BYTES + lane * 16);
+      for (int u = 0; u < 2 * U; u++)
+        kw[u] = *(const u2*)(p.kcodes + at + (size_t)(u / 2) * blocks * Q8_BYTES + n * Q8_BYTES + u % 2 * 512 + lane * 8);
 #pragma unroll
-      for (int u = 0; u < 2; u++) {
+      for (int u = 0; u < U; u++) vw[u] = *(const q8_u4*)(p.vcodes + at + (size_t)u * blocks * Q8_BYTES + n * Q8_BYTES + lane * 16);
+#pragma unroll
+      for (int u = 0; u < 2 * U; u++) {
         const int t = t0 + 8 * u, c = n * Q8_BLOCK + c8;
         float lo[4], hi[4];
         q8_floats<FMT>(kw[u][0], lo);
         q8_floats<FMT>(kw[u][1], hi);
-        a8 x;
+        q8_a8 x;
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] = from_f32<act_t>(t < there ? (e < 4 ? lo[e] : hi[e - 4]) * ks[u] : 0.f);
         act_t* to = p.k + out + (size_t)(sub * Q8_PIECE + t) * p.hd + c;
         if constexpr (WHOLE) {
-          if (c < p.hd) *(a8*)to = x;
+          if (c < p.hd) *(q8_a8*)to = x;
         } else {
 #pragma unroll
           for (int e = 0; e < 8; e++)
             if (c + e < p.hd) to[e] = x[e];
         }
       }
+      if constexpr (EIGHTS) {
+        // Odd rows of the first word change places with even rows of the second: row 0 has the first word's tokens 0 to 7, row 2 its
+        // tokens 8 to 15, rows 1 and 3 the second's.  The second word: the same channels' of the other piece, or the next 16 channels'.
 #pragma unroll
-      for (int b = 0; b < 4; b++) {
-        const int c = n * Q8_BLOCK + 16 * b + lane % 16, t = lane / 16 * 4;
-        float x[4];
-        q8_floats<FMT>(vw[b], x);
-        a4 y;
+        for (int b = 0; b < 4; b += PAIRS ? 1 : 2) {
+          const auto w = __builtin_amdgcn_permlane16_swap(vw[0][b], PAIRS ? vw[U - 1][b] : vw[0][(b + 1) % 4], false, false);
+          const int c = n * Q8_BLOCK + 16 * (PAIRS ? b : b + (row & 1)) + col;
+          float lo[4], hi[4];
+          q8_floats<FMT>(w[0], lo);
+          q8_floats<FMT>(w[1], hi);
+          q8_a8 y;
 #pragma unroll
-        for (int e = 0; e < 4; e++) y[e] = from_f32<act_t>(t + e < there ? x[e] * vs[e] : 0.f);
-        if (c < p.hd) {
-          if constexpr (TRANSPOSED) *(a4*)(p.v + out + (size_t)c * p.bs + sub * Q8_PIECE + t) = y;
-          else {
+          for (int e = 0; e < 8; e++) y[e] = from_f32<act_t>(first + e < there ? (e < 4 ? lo[e] : hi[e - 4]) * vs[e / 4][e % 4] : 0.f);
+          if (c < p.hd) *(q8_a8*)(p.v + out + (size_t)c * p.bs + sub * Q8_PIECE + first) = y;
+        }
+      } else {
 #pragma unroll
-            for (int e = 0; e < 4; e++) p.v[out + (size_t)(sub * Q8_PIECE + t + e) * p.hd + c] = y[e];
+        for (int b = 0; b < 4; b++) {
+          const int c = n * Q8_BLOCK + 16 * b + col, t = row * 4;
+          float x[4];
+          q8_floats<FMT>(vw[0][b], x);
+          q8_a4 y;
+#pragma unroll
+          for (int e = 0; e < 4; e++) y[e] = from_f32<act_t>(t + e < there ? x[e] * vs[0][e] : 0.f);
+          if (c < p.hd) {
+            if constexpr (TRANSPOSED) *(q8_a4*)(p.v + out + (size_t)c * p.bs + sub * Q8_PIECE + t) = y;
+            else {
+#pragma unroll
+              for (int e = 0; e < 4; e++) p.v[out + (size_t)(sub * Q8_PIECE + t + e) * p.hd + c] = y[e];
+            }
           }
         }
       }
@@ -593,13 +623,12 @@ __global__ __launch_bounds__(256, 2) void attention_q8_kernel(Q8Attention p) {
 #pragma unroll
       for (int s = 0; s < 2; s++) {
         const int c0 = 64 * j + 16 * g + 8 * s;
-        typedef act_t a8 __attribute__((ext_vector_type(8)));
-        a8 x;
+        q8_a8 x;
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] = from_f32<act_t>(0.f);
         if (col < heads) {
           if (p.q_whole) {
-            if (c0 < p.hd) x = *(const a8*)(row + c0);
+            if (c0 < p.hd) x = *(const q8_a8*)(row + c0);
           } else {
 #pragma unroll
             for (int e = 0; e < 8; e++)
@@ -1009,11 +1038,17 @@ int zk_cache_read_q8(const void* kcodes, const void* vcodes, const float* scales
   const long long pieces = ((max_ctx + (long long)bs - 1) / bs) * (bs / Q8_PIECE) * nkv * R;
   ZK_REQUIRE(pieces < (1ll << 30), "zk_cache_read_q8: too many pages");
   const int grid = (int)std::min<long long>((pieces + 3) / 4, Q8_READ_BLOCKS);
+  // pairs where they make whole runs of 64 bytes (four windows of 4,096 in pages of 32, 8 heads of 256: 56.8 -> 54.8 us)
+  auto launch = [&](auto f, auto t, auto w, auto u) {
+    read_q8_kernel<decltype(f)::value, decltype(t)::value, decltype(w)::value, decltype(u)::value><<<grid, 256, 0, (hipStream_t)stream>>>(p);
+  };
   q8_by_format(format, [&](auto f) {
-    q8_by_flag(v_transposed != 0, [&](auto t) {
-      q8_by_flag(hd % 8 == 0, [&](auto w) {
-        read_q8_kernel<decltype(f)::value, decltype(t)::value, decltype(w)::value><<<grid, 256, 0, (hipStream_t)stream>>>(p);
-      });
+    q8_by_flag(hd % 8 == 0, [&](auto w) {
+      if (!v_transposed) launch(f, std::false_type(), w, std::false_type());
+#if ZSE_ACT_BF16
+      else if (bs % (2 * Q8_PIECE) == 0) launch(f, std::true_type(), w, std::true_type());
+#endif
+      else launch(f, std::true_type(), w, std::false_type());
     });
   });
   return zk_launch_status("zk_cache_read_q8");
