@@ -908,9 +908,9 @@ static bool q8_meet(const void* a, long long a_ld, long long a_width, const void
 }
 
 // Blocks of a launch.  Written: the heads of four rows are dealt to as many blocks as that gives (4,092 rows of 32 heads and 2 x 16 of
-// 128 channels by 1,024, 2,048 and 4,096 blocks 43, 40 and 38 us; more work out the same angles).  Read back: waves that take
-// pieces in turn (64 pages of 8 heads in a range of 64,512 pieces by 2,048, 4,096 and 8,192 blocks 6.2, 8.1 and 10.4 us, empty ones
-// cost as much as others; 147,000 pieces that are all there 56.9, 56.3 and 56.2).
+// 128 channels by 1,024, 2,048 and 4,096 blocks 39.1, 37.0 and 36.6 us; more work out the same angles).  Read back: waves that take
+// pieces in turn (64 pages of 8 heads in a range of 64,512 pieces, one at a time, by 2,048, 4,096 and 8,192 blocks 8.0, 8.1 and 10.4 us:
+// empty blocks cost as much as others; 147,000 pieces that are all there 56.9, 56.3 and 56.2).
 #define Q8_WRITE_BLOCKS 4096
 #define Q8_READ_BLOCKS 2048
 
