@@ -136,6 +136,9 @@ __device__ __forceinline__ void q8_floats(unsigned codes, float (&x)[4]) {
 // head's largest magnitude is a maximum over the group's lanes, and four rows whose slots are four in a row from a multiple of four on
 // (a portion's) leave their values as whole words of the layout.  Such fours are taken together wherever they begin; the rows that
 // are in none (single tokens, a portion's ends) are taken as they come.  Sines and cosines of the four rows are worked out once, in LDS.
+// The channels that a lane's turn with come from the lane that has them, not from memory (4,092 rows as below 36.3 -> 33.0 us; 64 rows of
+// 16 heads of 256 out of three planes 7.2 -> 5.8, with the planes asked for together, out of six 8.7 -> 6.3).  Memory bounds the first
+// (3.6 TB/s), one wave's chain of waits the others; 72 registers instead of 80, for a seventh wave a SIMD, spill (36.6).
 template <bool SUMS>
 struct Q8Rows {
   const act_t* rows;
@@ -149,13 +152,28 @@ struct Q8Rows {
     for (int p = 1; p < sums; p++) x += (r + p * plane)[i];
     return from_f32<act_t>(x);
   }
-  __device__ __forceinline__ q8_a4 at4(int row, unsigned i) const {
-    if constexpr (!SUMS) return *(const q8_a4*)(rows + (size_t)row * ld + i);
-    else {
-      const float* r = planes + (size_t)row * ld;
-      q8_f4 x = *(const q8_f4*)(r + i);
-      for (int p = 1; p < sums; p++) x += *(const q8_f4*)(r + p * plane + i);
-      return q8_a4{from_f32<act_t>(x[0]), from_f32<act_t>(x[1]), from_f32<act_t>(x[2]), from_f32<act_t>(x[3])};
+  // four values of four rows; of planes three at a time, so that a turn is one wait for twelve loads (the last again where fewer are left)
+  __device__ __forceinline__ void at4(const int (&row)[4], unsigned i, q8_a4 (&to)[4]) const {
+    if constexpr (!SUMS) {
+#pragma unroll
+      for (int t = 0; t < 4; t++) to[t] = *(const q8_a4*)(rows + (size_t)row[t] * ld + i);
+    } else {
+      q8_f4 x[4];
+      for (int p = 0; p < sums; p += 3) {
+        q8_f4 y[3][4];
+#pragma unroll
+        for (int u = 0; u < 3; u++)
+#pragma unroll
+          for (int t = 0; t < 4; t++) y[u][t] = *(const q8_f4*)(planes + min(p + u, sums - 1) * plane + (size_t)row[t] * ld + i);
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+          x[t] = p == 0 ? y[0][t] : x[t] + y[0][t];
+          if (p + 1 < sums) x[t] += y[1][t];
+          if (p + 2 < sums) x[t] += y[2][t];
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 4; t++) to[t] = q8_a4{from_f32<act_t>(x[t][0]), from_f32<act_t>(x[t][1]), from_f32<act_t>(x[t][2]), from_f32<act_t>(x[t][3])};
     }
   }
 };
@@ -190,17 +208,30 @@ __device__ __forceinline__ float q8_largest(float v) {
   return larger(v, wave_dpp<ZSE_DPP_XOR1>(v));
 }
 
+// Another lane's four values.
+__device__ __forceinline__ q8_a4 q8_of_lane(q8_a4 x, int lane) {
+#ifdef __HIP_DEVICE_COMPILE__
+  typedef int words __attribute__((ext_vector_type(sizeof(q8_a4) / 4)));
+  words w = __builtin_bit_cast(words, x);
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(q8_a4) / 4); i++) w[i] = __builtin_amdgcn_ds_bpermute(lane * 4, w[i]);
+  return __builtin_bit_cast(q8_a4, w);
+#else
+  return x;
+#endif
+}
+
 // WHOLE: rows, heads and half the rotation are whole fours at addresses of whole fours.
 template <int FMT, int LANES, bool WHOLE, bool SUMS>
-__global__ __launch_bounds__(256, WHOLE ? 4 : 2) void write_q8_kernel(Q8Write<SUMS> p) {
+__global__ __launch_bounds__(256, WHOLE ? (SUMS ? 3 : 4) : 2) void write_q8_kernel(Q8Write<SUMS> p) {
 #ifdef __HIP_DEVICE_COMPILE__
   constexpr int HEADS = 256 / LANES;                // of a pass
   __shared__ q8_f4 s_sin[4][32], s_cos[4][32];
   const int lane = threadIdx.x & 63, sub = threadIdx.x / LANES, c0 = threadIdx.x % LANES * 4, half = p.rotary_dim / 2;
   const int blocks = q8_blocks(p.hd), pieces = p.bs / Q8_PIECE, t0 = blockIdx.x * 4;
   const bool rotated = c0 < p.rotary_dim, low = c0 < half, padded = c0 >= blocks * Q8_BLOCK;
-  // where a lane's channels, and those that they turn with, lie in a head; lanes without any read the head's first
-  const int own = c0 < p.hd ? c0 : 0, other = !rotated ? own : low ? c0 + half : c0 - half;
+  // where a lane's channels lie in a head (lanes without any read the head's first), and the lane that has those that they turn with
+  const int own = c0 < p.hd ? c0 : 0, mate_lane = !rotated ? lane : low ? lane + half / 4 : lane - half / 4;
   const int turn_at = rotated ? (low ? c0 : c0 - half) / 4 : 0;
   const int key_at = c0 / Q8_BLOCK * Q8_BYTES + c0 % Q8_BLOCK, value_at = c0 / Q8_BLOCK * Q8_BYTES + q8_value_at(0, c0 % Q8_BLOCK);
   const unsigned sign = low ? 0x80000000u : 0u;             // a - b turns where the lane holds the pair's first
@@ -242,12 +273,11 @@ __global__ __launch_bounds__(256, WHOLE ? 4 : 2) void write_q8_kernel(Q8Write<SU
     q8_a4 xr[4], yr[4];                              // a row's four channels, and those that they turn with: a pass ahead
     auto ask = [&](int base) {
       const unsigned head_at = min(base + sub, p.heads - 1) * p.hd;
+      if constexpr (WHOLE) {
+        p.from.at4(row, head_at + own, xr);
+      } else {
 #pragma unroll
-      for (int t = 0; t < 4; t++) {
-        if constexpr (WHOLE) {
-          xr[t] = p.from.at4(row[t], head_at + own);
-          yr[t] = p.from.at4(row[t], head_at + other);
-        } else {
+        for (int t = 0; t < 4; t++) {
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             const int c = c0 + e, mate = c >= p.rotary_dim ? c : c < half ? c + half : c - half;
@@ -273,6 +303,12 @@ __global__ __launch_bounds__(256, WHOLE ? 4 : 2) void write_q8_kernel(Q8Write<SU
         turned = true;
       }
       float x[4][4], y[4][4];
+      if constexpr (WHOLE) {
+        if (half > 0 && base < p.nh + p.nkv) {
+#pragma unroll
+          for (int t = 0; t < 4; t++) yr[t] = q8_of_lane(xr[t], mate_lane);
+        }
+      }
 #pragma unroll
       for (int t = 0; t < 4; t++)
 #pragma unroll
@@ -908,7 +944,7 @@ static bool q8_meet(const void* a, long long a_ld, long long a_width, const void
 }
 
 // Blocks of a launch.  Written: the heads of four rows are dealt to as many blocks as that gives (4,092 rows of 32 heads and 2 x 16 of
-// 128 channels by 1,024, 2,048 and 4,096 blocks 39.1, 37.0 and 36.6 us; more work out the same angles).  Read back: waves that take
+// 128 channels by 1,024, 2,048, 4,096 and 8,192 blocks 36.1, 33.9, 33.1 and 34.9 us; more work out the same angles).  Read back: waves that take
 // pieces in turn (64 pages of 8 heads in a range of 64,512 pieces, one at a time, by 2,048, 4,096 and 8,192 blocks 8.0, 8.1 and 10.4 us:
 // empty blocks cost as much as others; 147,000 pieces that are all there 56.9, 56.3 and 56.2).
 #define Q8_WRITE_BLOCKS 4096
