@@ -163,6 +163,25 @@ def test_written_otherwise(rt, what, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("hd,rotary", [(64, 8), (64, 48), (96, 64), (256, 64), (256, 248), (40, 16), (72, 10)])
+@pytest.mark.parametrize("planes", [0, 1, 2, 4, 5, 6, 7])
+def test_written_from_planes_and_turned_in_part(rt, planes, hd, rotary, dtype):
+    """The planes of a split product in the order of their numbers; heads of which a part turns, in fours of channels and not."""
+    rng = np.random.default_rng(planes + rotary)
+    nh, nkv, bs, form, T = 5, 2, 16, planes % 2, 11
+    before = random_cache(rng, 4, nkv, hd, bs, form)
+    inv_freq = (10000.0 ** (-np.arange(rotary // 2) * 2.0 / rotary)).astype(np.float32)
+    positions, slots = np.arange(T) + 900, np.concatenate([21 + np.arange(9), [40, 60]])
+    parts = rng.standard_normal((max(planes, 1), T, (nh + 2 * nkv) * hd)).astype(np.float32)
+    rows = parts[0]
+    for x in parts[1:]:
+        rows = rows + x
+    rows = rounded(rows, dtype)
+    q, got = write(rt, dtype, before, rows, positions, slots, inv_freq, rotary, nh, planes=parts if planes else None)
+    check_written(before, got, q, rows.astype(np.float64), positions, slots, inv_freq, rotary, nh, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
 @pytest.mark.parametrize("form", [0, 1])
 def test_written_from_zeros_and_what_is_not_finite(rt, form, dtype):
     rng = np.random.default_rng(2)
