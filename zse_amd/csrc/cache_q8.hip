@@ -870,7 +870,8 @@ __global__ __launch_bounds__(256, 2) void attention_q8_kernel(Q8Attention p) {
 // behind its chunks is never used).
 template <int NB>
 __global__ __launch_bounds__(256) void attention_q8_join_kernel(Q8Attention p, int splits) {
-  constexpr int LANES = NB * 16, GROUPS = 256 / LANES, AHEAD = 8;
+  constexpr int LANES = NB * 16, GROUPS = 256 / LANES, AHEAD = GROUPS > 8 ? 4 : 8;
+  static_assert(AHEAD * GROUPS <= 64, "the first round's factors are one wave's lanes");
   __shared__ float s_o[GROUPS][NB * 64];
   const int head = blockIdx.x, r = blockIdx.y, lane = threadIdx.x & 63, group = min((int)threadIdx.x / LANES, GROUPS - 1), at = threadIdx.x % LANES;
   const size_t row = ((size_t)r * p.nh + head) * splits;
