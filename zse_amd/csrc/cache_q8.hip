@@ -967,11 +967,13 @@ static void q8_by_flag(bool flag, F go) {
 // channels): one request of 4,000 keys 10.8, 12.8, 18.9; 64 of them 98.6, 93.7, 91.4; one of 16,000 15.6, 15.3, 20.8; eight of
 // them 56.3, 49.8, 47.9; one of 60,000 45.1, 33.5, 28.3.  32-bit products take eight times as long for as many keys: by 128, 256
 // and 512, 8 heads over 2 of 128, three requests of up to 700 keys 10.2, 12.9, 19.7; 8 over 4 of 256, one of 16,000 29.4, 25.1, 33.9.
+#define Q8_WIDE 8192                  // tokens of a table from which chunks are longer
+#define Q8_WIDER 32768
 static int q8_chunk(long long table_tokens) {
 #if ZSE_ACT_BF16
-  return table_tokens < 8192 ? 256 : table_tokens < 32768 ? 512 : 1024;
+  return table_tokens < Q8_WIDE ? 256 : table_tokens < Q8_WIDER ? 512 : 1024;
 #else
-  return table_tokens < 8192 ? 128 : 256;
+  return table_tokens < Q8_WIDE ? 128 : 256;
 #endif
 }
 
@@ -1091,11 +1093,15 @@ int zk_cache_read_q8(const void* kcodes, const void* vcodes, const float* scales
   return zk_launch_status("zk_cache_read_q8");
 }
 
-// Bytes of workspace of zk_attention_q8 for R requests of up to max_ctx tokens whose table reaches table_tokens (more of either is
-// more: a caller may ask for its largest).
+// Bytes of workspace of zk_attention_q8 for up to R requests of up to max_ctx tokens in tables that reach up to table_tokens: what is
+// enough for the largest of each is enough for less.  (A narrower table may need more: its chunks are shorter.)
 size_t zk_attention_q8_workspace(int R, int nh, int hd, int max_ctx, int table_tokens) {
   if (R <= 0 || nh <= 0 || hd <= 0 || hd > 256 || max_ctx <= 0) return 0;
-  return (size_t)R * nh * q8_splits(max_ctx, 0, q8_chunk(table_tokens)) * (q8_blocks(hd) * Q8_BLOCK + 2) * sizeof(float);
+  const int widest = std::max(max_ctx, table_tokens);
+  int splits = q8_splits(max_ctx, 0, q8_chunk(widest));
+  for (const int narrower : {Q8_WIDE - 1, Q8_WIDER - 1})         // the widest of shorter chunks
+    if (narrower < widest) splits = std::max(splits, q8_splits(std::min(max_ctx, narrower), 0, q8_chunk(narrower)));
+  return (size_t)R * nh * splits * (q8_blocks(hd) * Q8_BLOCK + 2) * sizeof(float);
 }
 
 // Attention of one token a request, the last of its ctx_len[r], over its cache: z_j = scale q.k_j (softcap > 0: softcap
