@@ -1166,7 +1166,10 @@ int zk_attention_q8(const void* q, int q_stride, const void* kcodes, const void*
   p.rest = softcap > 0.f ? (float)(softcap * log2e - p.c2) : (float)(scale * log2e - p.k1);
   const int group = nh / nkv, tiles = (group + 15) / 16;
   const dim3 grid(nkv * tiles, R, splits);
-  // codes past the caches where one block alone reads them and the launch may pass through more than the memory side's cache holds
+  // Codes past the caches where one block alone reads them and R requests of max_ctx keys are more than the memory side's cache holds.  A
+  // window is not taken off: what it leaves of a layer may fit, what all layers of a step read does not (behind a window of 4,096, one layer
+  // over and over / eight in turn: 8 requests of 20,000, 4 heads of 256, 20.9 / 22.5 us past the caches, 20.3 / 24.1 through them; 4 of 60,000, 8
+  // heads of 128, 17.6 / 19.2 and 16.9 / 19.1).
   const bool once = tiles == 1 && (double)R * max_ctx * nkv * (2 * blocks * Q8_BLOCK + 8) > 256.0 * (1 << 20);
   const size_t lds = (size_t)4 * std::min(group, 16) * (blocks * Q8_BLOCK + 4) * sizeof(float);
 #define Q8_KERNEL(FMT, NB, CAP, DIRECT) (once ? attention_q8_kernel<FMT, NB, CAP, DIRECT, true> : attention_q8_kernel<FMT, NB, CAP, DIRECT, false>)
