@@ -271,7 +271,7 @@ class PagedAttention(Part):
                                  g.page_size, pages, cache.format, ctx.stream)
         o = ctx.alloc((T, nh * hd))
         cap = float(s.softcap) if s.softcap else 0.0
-        win = int(s.window) if s.window else 0
+        win = int(s.window) if s.window and s.window < ctx.max_ctx else 0        # (more than there is: sums with it stay in 32 bits)
         n, single = ctx.n_multi, ctx.R - ctx.n_multi        # requests of several tokens come first
         first = T - single
         if n:
