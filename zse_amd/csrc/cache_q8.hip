@@ -937,11 +937,10 @@ static int q8_refuses(const char* who, const void* kcodes, const void* vcodes, c
 #define Q8_REQUIRE_CACHE(who) \
   if (const int rc = q8_refuses(who, kcodes, vcodes, scales, nkv, hd, bs, num_pages, format)) return rc
 
-// Whether two ranges of values of the activations' type meet: ``rows`` rows of ``width``, ``ld`` apart.
-static bool q8_meet(const void* a, long long a_ld, long long a_width, const void* b, long long b_ld, long long b_width, long long rows) {
-  const uintptr_t a0 = (uintptr_t)a, a1 = a0 + ((rows - 1) * a_ld + a_width) * sizeof(act_t);
-  const uintptr_t b0 = (uintptr_t)b, b1 = b0 + ((rows - 1) * b_ld + b_width) * sizeof(act_t);
-  return a0 < b1 && b0 < a1;
+// Bytes from the first to the last of ``rows`` rows of ``width`` values of the activations' type, ``ld`` apart.
+static size_t q8_span(long long ld, long long width, long long rows) { return ((rows - 1) * ld + width) * sizeof(act_t); }
+static bool q8_meet(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+  return (uintptr_t)a < (uintptr_t)b + b_bytes && (uintptr_t)b < (uintptr_t)a + a_bytes;
 }
 
 // Blocks of a launch.  Written: the heads of four rows are dealt to as many blocks as that gives (4,092 rows of 32 heads and 2 x 16 of
@@ -993,7 +992,7 @@ size_t zk_cache_q8_bytes(int num_pages, int nkv, int hd, int bs) {
 
 // Rotates the queries and keys of T rows (query heads, key heads, value heads, ``ld`` values apart, or ``sums`` float planes
 // [T][(nh + 2 nkv) hd] to add up, then rounded to the activations' type), stores the queries in rows of ``ldq`` values at q_out
-// (qkv itself, where ldq is ld, is allowed) and the keys and values in 8 bits at slot_map[t] = page * bs + offset.  A slot below
+// (qkv itself, where ldq is ld, is allowed; not the planes) and the keys and values in 8 bits at slot_map[t] = page * bs + offset.  A slot below
 // zero or behind the last page is not stored; the slots of one call are distinct.  slot_map may be null, nkv zero: queries only.
 int zk_rope_cache_write_q8(const void* qkv, int ld, const float* planes, int sums, void* q_out, int ldq, const int* positions,
                            const int* slot_map, const float* inv_freq, int rotary_dim, void* kcodes, void* vcodes, void* scales, int T,
@@ -1013,8 +1012,11 @@ int zk_rope_cache_write_q8(const void* qkv, int ld, const float* planes, int sum
              "zk_rope_cache_write_q8: null or misaligned argument");
   const int width = (nh + 2 * nkv) * hd, blocks = q8_blocks(hd);
   const bool partial = sums > 0;
-  ZK_REQUIRE(partial || (q_out == qkv && ldq == ld) || !q8_meet(qkv, ld, width, q_out, ldq, (long long)nh * hd, T),
+  const size_t q_bytes = q8_span(ldq, (long long)nh * hd, T);
+  ZK_REQUIRE(partial || (q_out == qkv && ldq == ld) || !q8_meet(qkv, q8_span(ld, width, T), q_out, q_bytes),
              "zk_rope_cache_write_q8: queries may go where they came from, in rows as far apart, or elsewhere");
+  ZK_REQUIRE(!partial || !q8_meet(planes, (size_t)sums * T * width * sizeof(float), q_out, q_bytes),
+             "zk_rope_cache_write_q8: queries over the partial sums");
   const int row = partial ? width : ld, heads = slot_map ? nh + 2 * nkv : nh;
   const bool whole = hd % 4 == 0 && rotary_dim % 8 == 0 && row % 4 == 0 && ldq % 4 == 0 && (uintptr_t)q_out % (4 * sizeof(act_t)) == 0 &&
                      (partial || (uintptr_t)qkv % (4 * sizeof(act_t)) == 0);
@@ -1122,7 +1124,7 @@ int zk_attention_q8(const void* q, int q_stride, const void* kcodes, const void*
   ZK_REQUIRE(softcap >= 0.f, "zk_attention_q8: softcap must not be negative");
   if (R == 0) return 0;
   ZK_REQUIRE(q && out && ctx_len && (block_table || max_ctx == 0), "zk_attention_q8: null argument");
-  ZK_REQUIRE(!q8_meet(q, q_stride, (long long)nh * hd, out, (long long)nh * hd, (long long)nh * hd, R), "zk_attention_q8: results over queries");
+  ZK_REQUIRE(!q8_meet(q, q8_span(q_stride, (long long)nh * hd, R), out, (size_t)R * nh * hd * sizeof(act_t)), "zk_attention_q8: results over queries");
   if (window >= max_ctx) window = 0;                   // (sums of ctx and window stay in 32 bits)
   Q8Attention p;
   p.chunk = q8_chunk((long long)max_blocks * bs);
