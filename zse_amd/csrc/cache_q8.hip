@@ -1121,7 +1121,7 @@ int zk_attention_q8(const void* q, int q_stride, const void* kcodes, const void*
   ZK_REQUIRE(max_ctx <= 1 << 30, "zk_attention_q8: contexts of more than 2^30 tokens");
   ZK_REQUIRE(max_ctx <= (long long)max_blocks * bs, "zk_attention_q8: contexts longer than the table");
   ZK_REQUIRE((long long)num_pages * nkv * 2 * (bs / Q8_PIECE) < (1ll << 31), "zk_attention_q8: too many pages");
-  ZK_REQUIRE(softcap >= 0.f, "zk_attention_q8: softcap must not be negative");
+  ZK_REQUIRE(softcap >= 0.f && softcap <= FLT_MAX, "zk_attention_q8: softcap must be finite and not negative (0: no cap)");
   if (R == 0) return 0;
   ZK_REQUIRE(q && out && ctx_len && (block_table || max_ctx == 0), "zk_attention_q8: null argument");
   ZK_REQUIRE(!q8_meet(q, q8_span(q_stride, (long long)nh * hd, R), out, (size_t)R * nh * hd * sizeof(act_t)), "zk_attention_q8: results over queries");
