@@ -137,8 +137,9 @@ __device__ __forceinline__ void q8_floats(unsigned codes, float (&x)[4]) {
 // (a portion's) leave their values as whole words of the layout.  Such fours are taken together wherever they begin; the rows that
 // are in none (single tokens, a portion's ends) are taken as they come.  Sines and cosines of the four rows are worked out once, in LDS.
 // The channels that a lane's turn with come from the lane that has them, not from memory (4,092 rows as below 36.3 -> 33.0 us; 64 rows of
-// 16 heads of 256 out of three planes 7.2 -> 5.8, with the planes asked for together, out of six 8.7 -> 6.3).  Memory bounds the first
-// (3.6 TB/s), one wave's chain of waits the others; 72 registers instead of 80, for a seventh wave a SIMD, spill (36.6).
+// 16 heads of 256 out of three planes 7.2 -> 5.8, with the planes asked for together, out of six 8.7 -> 6.3).  The first moves
+// 3.6 TB/s, with 1.22 M write requests for 0.79 M lines of 64 bytes (values': four bytes a store at a stride of 16); one wave's chain of waits
+// bounds the others; 72 registers instead of 80, for a seventh wave a SIMD, spill (36.6).
 template <bool SUMS>
 struct Q8Rows {
   const act_t* rows;
@@ -1107,7 +1108,8 @@ size_t zk_attention_q8_workspace(int R, int nh, int hd, int max_ctx, int table_t
 }
 
 // Attention of one token a request, the last of its ctx_len[r], over its cache: z_j = scale q.k_j (softcap > 0: softcap
-// tanh(z_j / softcap)) for j from max(0, ctx - window) on (all without a window), out = sum softmax(z)_j v_j.  q: row r at r * q_stride;
+// tanh(z_j / softcap)) for j from max(0, ctx - window) on (all without a window), out = sum softmax(z)_j v_j.  In 16 bits a capped
+// score is off by up to softcap 2^-20: caps are tens, not hundred thousands.  q: row r at r * q_stride;
 // out: rows of nh * hd, apart from q.  A request without keys gets zeros, and a page that the table does not name (below zero, or not below
 // num_pages) has none.
 int zk_attention_q8(const void* q, int q_stride, const void* kcodes, const void* vcodes, const float* scales, const int* block_table,
