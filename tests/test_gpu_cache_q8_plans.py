@@ -156,3 +156,32 @@ def test_every_generated_id_is_one_of_the_largest(monkeypatch, tiny_folders, dty
             short = z.max(axis=1) - z[np.arange(20), out]
             assert (short <= 2 * off_by(dtype, z, rounding)).all(), (blocks, len(p), short.max(), rounding)
             assert np.median(short) == 0
+
+
+@pytest.mark.parametrize("cache_dtype", ["int8", "float8_e4m3"])
+def test_company_leaves_a_requests_bits_in_32_bits(tiny_folders, cache_dtype):
+    """Cut alike, alone and beside others that come, decode and end."""
+    from gpu_util import make_runner
+    from zse_amd.engine.runner import StepEntry
+    rng = np.random.default_rng(1)
+    tokens = rng.integers(0, 512, 90).tolist()
+    cuts = [30, 1, 1, 20, 1, 1, 1, 12] + [1] * 10
+    got = []
+    for company in (False, True):
+        runner = make_runner(tiny_folders[("A", "float32")], "float32", page_size=16, num_pages=60, max_seqs=6, max_batch_tokens=256, max_model_len=256,
+                             use_graphs=True, cache_dtype=cache_dtype)
+        rows, at = [], 0
+        for i, n in enumerate(cuts):
+            entries = [StepEntry("r", tokens[at:at + n], list(range(n)))]
+            at += n
+            if company:
+                if i == 9:
+                    runner.finish("x")
+                entries = ([StepEntry("x", tokens[:40] if i == 0 else [i], [0])] if i < 9 else []) + entries
+                entries += [StepEntry(j, [7 + i, j, 3][:1 + (i + j) % 3], []) for j in range(min(i, 4))]
+            z = runner.step(entries)
+            first = 1 if company and i < 9 else 0
+            rows.append(z[first:first + n])
+        runner.close()
+        got.append(np.concatenate(rows))
+    assert np.array_equal(*got)
